@@ -139,6 +139,95 @@ int vrt_q8_quantize(vrt_ctx* ctx, const float* x, uint64_t n, uint32_t variant, 
 /* GgufFile::read_q8_0_row dequant (src/gguf.cpp:620-635) on the GPU: n_blocks -> floats. */
 int vrt_q8_dequantize(vrt_ctx* ctx, const void* blocks, uint64_t n_blocks, float* out);
 
+/* ---- 8-bit key/value cache ------------------------------------------------------------ */
+/* No counterpart in the reference (its KV cache is fp32, one sequence; src/gemma3.cpp:546-600). A
+ * cache holds the keys and values of max_seqs sequences ("regions") of kv_heads heads in int8, with
+ * one scale for the keys and one for the values of every VRT_KV8_BLOCK consecutive positions of a
+ * head: s = fl32(max|x| / 127), q = x / s rounded to the nearest integer (ties to even), and the
+ * cache stands for fl32(q s). The positions of a block that is not full yet count in fp32, and are
+ * rounded once, when the block fills: in which pieces a sequence is appended does not matter.
+ * A block with a value that is not finite stands for NaN.
+ *
+ * The memory is the caller's (vrt_alloc, at least vrt_kv8_cache_bytes, 256-byte aligned); its layout
+ * is the library's own. Nothing else is kept: sequences' lengths are the caller's, and every call
+ * names the positions it means. Position p occupies block (p / 32) % ceil(max_ctx / 32) of its region,
+ * so longer sequences run as a ring under a window.
+ *
+ * k, v, q and out are device arrays of rows, one row per position: row stride in floats (0: packed), a
+ * multiple of 4, 16-byte aligned. A call's rows are those of its sequences one after another. The
+ * arrays vrt_kv8_rows / vrt_kv8_move are on the host and read before the call returns. Calls are
+ * stream-ordered, allocate nothing and can be captured; a replay repeats the positions of the capture.
+ * Every argument is checked before any launch. */
+#define VRT_KV8_BLOCK 32
+#define VRT_KV8_MAX_SEQS 64      /* sequences of one call */
+#define VRT_KV8_MAX_CTX (1u << 26)
+
+typedef struct vrt_kv8_cache {
+    void* data;            /* device memory */
+    uint64_t bytes;        /* its size */
+    uint32_t max_seqs;     /* regions */
+    uint32_t max_ctx;      /* positions a region holds (rounded up to whole blocks) */
+    uint32_t kv_heads;
+    uint32_t head_dim;     /* 4..256, a multiple of 4 */
+} vrt_kv8_cache;
+
+/* Positions pos .. pos + n - 1 of region seq (n may be 0). prefix: see vrt_kv8_attend. */
+typedef struct vrt_kv8_rows {
+    uint32_t seq, pos, n, prefix;
+} vrt_kv8_rows;
+
+/* Bytes of a cache of these sizes (cache->data and cache->bytes are not read). */
+int vrt_kv8_cache_bytes(const vrt_kv8_cache* cache, uint64_t* bytes);
+
+/* Writes the keys and values of n_seqs (1..VRT_KV8_MAX_SEQS) distinct regions' positions: rows of
+ * [kv_heads][head_dim]. pos is the sequence's length, or less to take it back: to any multiple of 32, or to a position
+ * inside a block b as long as no position of block b + 2 has been written since those of b before it. One call writes at
+ * most as many blocks as a region has. */
+int vrt_kv8_append(vrt_ctx* ctx, const vrt_kv8_cache* cache, const vrt_kv8_rows* rows, uint32_t n_seqs, const float* k,
+                   const float* v, uint64_t kv_stride);
+
+/* What the cache stands for at the given positions, as fp32 rows; lens[i] (host; NULL: pos + n) is the
+ * length of sequence rows[i].seq. */
+int vrt_kv8_read(vrt_ctx* ctx, const vrt_kv8_cache* cache, const vrt_kv8_rows* rows, uint32_t n_seqs, const uint32_t* lens,
+                 float* k, float* v, uint64_t kv_stride);
+
+typedef struct vrt_kv8_attn {
+    uint32_t heads;        /* query heads, a multiple of kv_heads: head h reads kv head h / (heads / kv_heads) */
+    uint32_t window;       /* positions a query sees back, its own included (0: all) */
+    float scale;           /* of the scores q . k */
+    float softcap;         /* > 0: scores become softcap tanh(score / softcap); 0: off */
+} vrt_kv8_attn;
+
+/* Attention of the last n positions of each sequence over its cache (which holds all pos + n of
+ * them: append first): q and out are rows of [heads][head_dim]. The query at position i sees position j
+ * if j < prefix, or if j <= i and i - j < window (a prefix is seen by every query: the bidirectional part of a
+ * prompt, or positions that stay in sight past a window). The softmax runs in fp32.
+ * A key or value that is not finite (in a full block: any of the block) makes the outputs of the queries that see it NaN.
+ * weights_out (may be NULL): [max_seqs][kv_heads][max_ctx] floats; of the regions of the call, the entries of
+ * positions 0 .. pos + n - 1 become weights_in's (NULL, or the call's own positions: 0) plus the softmax weights that the
+ * position got in this call, over all queries and the heads of its group. weights_in may be weights_out. Needs
+ * pos + n <= max_ctx.
+ * workspace: at least vrt_kv8_attend_workspace bytes of device memory, 256-byte aligned, in use until the call's
+ * work is done (two calls that may overlap, as replays of two captured graphs may, need one each). NULL where that is 0. */
+int vrt_kv8_attend(vrt_ctx* ctx, const vrt_kv8_cache* cache, const vrt_kv8_attn* attn, const vrt_kv8_rows* rows,
+                   uint32_t n_seqs, const float* q, uint64_t q_stride, float* out, uint64_t out_stride,
+                   const float* weights_in, float* weights_out, void* workspace, uint64_t workspace_bytes);
+/* The workspace of such a call; scored: with weights_out. */
+int vrt_kv8_attend_workspace(const vrt_kv8_cache* cache, const vrt_kv8_attn* attn, const vrt_kv8_rows* rows,
+                             uint32_t n_seqs, uint32_t scored, uint64_t* bytes);
+
+/* Eviction: sequence src of len positions becomes sequence dst of keep positions. Each head keeps the last
+ * `recent` positions and, of the others, the keep - recent with the largest weights (vrt_argmax's order: larger wins, NaN
+ * never, equal weights: the lower position), in their old order; the kept values (what the cache stands
+ * for) are put into blocks as vrt_kv8_append does. weights [max_seqs][kv_heads][max_ctx] is read in region src and written
+ * in region dst (keep entries); kept [n][kv_heads][kept_stride] receives the kept positions. recent <= keep <= len <=
+ * max_ctx; the dst regions are distinct and none is a src. */
+typedef struct vrt_kv8_move {
+    uint32_t src, dst, len, keep, recent;
+} vrt_kv8_move;
+int vrt_kv8_evict(vrt_ctx* ctx, const vrt_kv8_cache* cache, const vrt_kv8_move* moves, uint32_t n, float* weights,
+                  uint32_t* kept, uint64_t kept_stride);
+
 /* ---- Gemma 3 executor --------------------------------------------------------------- */
 
 /* Gemma3Config, include/vortexrt/gemma3.hpp:19-33. */

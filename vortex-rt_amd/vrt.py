@@ -69,6 +69,15 @@ class G3Desc(C.Structure):
                 ("eos_token_id", C.c_uint32)]
 
 
+class Kv8CacheDesc(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("bytes", C.c_uint64), ("max_seqs", C.c_uint32), ("max_ctx", C.c_uint32),
+                ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32)]
+
+
+class Kv8Attn(C.Structure):
+    _fields_ = [("heads", C.c_uint32), ("window", C.c_uint32), ("scale", C.c_float), ("softcap", C.c_float)]
+
+
 # Every symbol include/vrt_hip.h declares, with its ctypes signature.
 _P, _U32, _U64, _I, _F = C.c_void_p, C.c_uint32, C.c_uint64, C.c_int, C.c_float
 SIGNATURES = {
@@ -94,6 +103,12 @@ SIGNATURES = {
     "vrt_argmax": (_I, [_P, _P, _U32, _P]),
     "vrt_q8_quantize": (_I, [_P, _P, _U64, _U32, _P]),
     "vrt_q8_dequantize": (_I, [_P, _P, _U64, _P]),
+    "vrt_kv8_cache_bytes": (_I, [_P, C.POINTER(_U64)]),
+    "vrt_kv8_append": (_I, [_P, _P, _P, _U32, _P, _P, _U64]),
+    "vrt_kv8_read": (_I, [_P, _P, _P, _U32, _P, _P, _P, _U64]),
+    "vrt_kv8_attend_workspace": (_I, [_P, _P, _P, _U32, _U32, C.POINTER(_U64)]),
+    "vrt_kv8_attend": (_I, [_P, _P, _P, _P, _U32, _P, _U64, _P, _U64, _P, _P, _P, _U64]),
+    "vrt_kv8_evict": (_I, [_P, _P, _P, _U32, _P, _P, _U64]),
     "vrt_g3_create": (_I, [_P, C.POINTER(G3Desc), C.POINTER(_P)]),
     "vrt_g3_destroy": (_I, [_P]),
     "vrt_g3_reset": (_I, [_P]),
@@ -271,6 +286,84 @@ def q8_quantize(ctx, x: DeviceBuffer, n: int, variant: int, out: DeviceBuffer):
 
 def q8_dequantize(ctx, blocks: DeviceBuffer, nblocks: int, out: DeviceBuffer):
     check(lib().vrt_q8_dequantize(ctx.h, blocks.ptr, nblocks, out.ptr))
+
+
+# ---- 8-bit key/value cache -------------------------------------------------------------------
+
+class Kv8Cache:
+    """Keys and values of max_seqs sequences in int8 with a scale per block of 32 positions and head
+    (vrt_kv8_*). rows: uint32 [n, 4] of (seq, pos, n, prefix), one line per sequence of a call; k, v, q,
+    out and weights are device buffers (or addresses). The cache and the attention's workspace are device memory of the context."""
+
+    def __init__(self, ctx: Context, max_seqs: int, max_ctx: int, kv_heads: int, head_dim: int):
+        self.ctx = ctx
+        self.desc = Kv8CacheDesc(None, 0, max_seqs, max_ctx, kv_heads, head_dim)
+        n = C.c_uint64()
+        check(lib().vrt_kv8_cache_bytes(C.byref(self.desc), C.byref(n)))
+        self.buf = ctx.alloc(n.value)
+        self.desc.data, self.desc.bytes = self.buf.ptr, n.value
+        self._ref = C.byref(self.desc)
+        self._ws = None
+
+    def close(self):
+        for b in (self.buf, self._ws):
+            if b is not None:
+                b.free()
+        self.buf = self._ws = None
+
+    @staticmethod
+    def _table(a, width):
+        a = np.ascontiguousarray(a, dtype=np.uint32)
+        if a.ndim != 2 or a.shape[1] != width:
+            raise ValueError(f"expected lines of {width} numbers")
+        return a
+
+    def _alive(self):
+        if self.buf is None or self.buf.ptr is None:
+            raise RuntimeError("the cache is closed")
+
+    def append(self, rows, k, v, stride: int = 0):
+        self._alive()
+        r = self._table(rows, 4)
+        check(lib().vrt_kv8_append(self.ctx.h, self._ref, ptr(r), len(r), ptr(k), ptr(v), stride))
+
+    def read(self, rows, k, v, lens=None, stride: int = 0):
+        """The values the cache stands for; lens: the sequences' lengths (default pos + n)."""
+        self._alive()
+        r = self._table(rows, 4)
+        n = None if lens is None else np.ascontiguousarray(lens, dtype=np.uint32)
+        if n is not None and n.shape != (len(r),):
+            raise ValueError("one length per sequence")
+        check(lib().vrt_kv8_read(self.ctx.h, self._ref, ptr(r), len(r), ptr(n), ptr(k), ptr(v), stride))
+
+    def workspace_bytes(self, rows, heads: int, scale: float, softcap: float = 0.0, window: int = 0, scored: bool = False) -> int:
+        r = self._table(rows, 4)
+        at, n = Kv8Attn(heads, window, scale, softcap), C.c_uint64()
+        check(lib().vrt_kv8_attend_workspace(self._ref, C.byref(at), ptr(r), len(r), int(scored), C.byref(n)))
+        return n.value
+
+    def attend(self, rows, q, out, heads: int, scale: float, softcap: float = 0.0, window: int = 0, weights_in=None,
+               weights_out=None, q_stride: int = 0, out_stride: int = 0, workspace: DeviceBuffer | None = None):
+        """Attention of the rows' positions. workspace: the cache's own unless given, grown as calls need it
+        (a captured call needs one that no larger call replaces)."""
+        self._alive()
+        r = self._table(rows, 4)
+        at = Kv8Attn(heads, window, scale, softcap)
+        n = C.c_uint64()
+        check(lib().vrt_kv8_attend_workspace(self._ref, C.byref(at), ptr(r), len(r), int(weights_out is not None), C.byref(n)))
+        ws = workspace if workspace is not None else self._ws
+        if workspace is None and n.value and (ws is None or ws.nbytes < n.value):
+            if ws is not None:
+                ws.free()   # waits for the calls that use it
+            ws = self._ws = self.ctx.alloc(n.value)
+        check(lib().vrt_kv8_attend(self.ctx.h, self._ref, C.byref(at), ptr(r), len(r), ptr(q), q_stride, ptr(out), out_stride,
+                                   ptr(weights_in), ptr(weights_out), ptr(ws), 0 if ws is None else ws.nbytes))
+
+    def evict(self, moves, weights, kept, kept_stride: int):
+        """moves: uint32 [n, 5] of (src, dst, len, keep, recent)."""
+        self._alive()
+        m = self._table(moves, 5)
+        check(lib().vrt_kv8_evict(self.ctx.h, self._ref, ptr(m), len(m), ptr(weights), ptr(kept), kept_stride))
 
 
 # ---- Gemma 3 executor ----------------------------------------------------------------------
