@@ -410,6 +410,17 @@ int vrt_g3_get_option(vrt_g3* g3, uint32_t option, uint32_t* value);
  * position 0, as the reference resets its cache. */
 typedef struct vrt_g3_batch vrt_g3_batch;
 int vrt_g3_batch_create(vrt_g3* g3, uint32_t max_seqs, uint32_t max_ctx, vrt_g3_batch** out);
+/* The same over 8-bit caches (vrt_kv8_*: a quarter of the memory, and of the bytes a step reads of it):
+ * keys and values after QK-norm and RoPE are held as int8 with a scale per 32 positions, the positions of a
+ * block that is not full in fp32. evict = 1: the blocks that attend to every position also accumulate each position's softmax
+ * weights, and vrt_g3_batch_evict shortens a sequence's caches by them, so that a conversation goes on past max_ctx
+ * entries (to context_length positions). */
+int vrt_g3_batch_create_kv8(vrt_g3* g3, uint32_t max_seqs, uint32_t max_ctx, uint32_t evict, vrt_g3_batch** out);
+/* vrt_kv8_evict over the sequence's caches: `keep` of their entries stay, the last `recent` among them (recent <= keep,
+ * 1 <= keep <= vrt_g3_batch_length). Positions go on counting; blocks with a sliding window keep their window. */
+int vrt_g3_batch_evict(vrt_g3_batch* b, uint32_t seq, uint32_t keep, uint32_t recent);
+/* Entries of the sequence's caches: its position, or fewer after an eviction. A step needs one below max_ctx. */
+int vrt_g3_batch_length(vrt_g3_batch* b, uint32_t seq, uint32_t* len);
 /* The batch reads its executor's weights and launches on its context's stream: destroy it
  * before the executor (vrt_g3_destroy refuses while it is alive). */
 int vrt_g3_batch_destroy(vrt_g3_batch* b);

@@ -12,7 +12,8 @@
 //                 QK-norm, RoPE at the row's position, KV append to the row's sequence, attention;
 //                 else k_bd_attn, per (history chunk, row), the same with a chunk of the attention
 //                 (max, sum, weighted V per head), and k_bd_merge, per (head, row): the chunks
-//                 combined, as f16 hi/lo GEMM input
+//                 combined, as f16 hi/lo GEMM input. Over 8-bit caches: k_bd_qk, then the append and the attention of
+//                 vrt_kv8.hip
 //   GEMM          O projection; k_pf_norm_w (post-attention norm + residual + FFN norm)
 //   GEMM          gelu_tanh(gate) * up (with its norm up to 16 rows); GEMM down projection
 // then the final residual + output norm (k_pf_norm_w), the logits of the n rows against the
@@ -29,6 +30,7 @@
 #include "vrt_g3_internal.hpp"
 #include "vrt_gemm.hpp"
 #include "vrt_internal.hpp"
+#include "vrt_kv8.hpp"
 #include "vrt_q8_device.hpp"
 
 namespace vrt {
@@ -444,6 +446,63 @@ __global__ void __launch_bounds__(kBdThreads) k_bd_merge(BdAttn A) {
     }
 }
 
+// The rows of a step for the 8-bit cache: q with QK-norm and RoPE at the row's position [n][H hd], k the same, v as it is
+// [n][hd]. One wave per (head, row): lane l has dims l + 64 e (the order of operations of k_bd_attn).
+struct BdQk {
+    const float* qkv;
+    uint64_t sstride;
+    uint32_t nsplit, H, hd, n;
+    const uint32_t* pos;
+    const float* q_norm;
+    const float* k_norm;
+    const float* cos_t;
+    const float* sin_t;
+    float eps;
+    float* q;
+    float* k;
+    float* v;
+};
+__global__ void __launch_bounds__(kBdThreads) k_bd_qk(BdQk A) {
+#pragma clang fp contract(off)
+    __shared__ float s_x[kBdThreads / 64u][256];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, b = blockIdx.y, H = A.H, hd = A.hd, half = hd >> 1;
+    const uint32_t h = blockIdx.x * (kBdThreads / 64u) + wave;
+    if (h >= H + 2u) return;   // whole waves; no barrier follows
+    const float* src = A.qkv + static_cast<uint64_t>(b) * (H + 2u) * hd + h * hd;
+    const uint32_t p = A.pos[b];
+    float* x = s_x[wave];
+    float v[4], wv[4], cs[4], sn[4];
+    uint32_t ic[4], ei[4];
+    const float* w = h < H ? A.q_norm : A.k_norm;
+    double ss = 0.0;
+#pragma unroll
+    for (uint32_t e = 0; e < 4u; ++e) {
+        ic[e] = min(lane + 64u * e, hd - 1u);
+        ei[e] = ic[e] < half ? ic[e] : ic[e] - half;
+        cs[e] = A.cos_t[static_cast<uint64_t>(p) * half + ei[e]];
+        sn[e] = A.sin_t[static_cast<uint64_t>(p) * half + ei[e]];
+        wv[e] = w[ic[e]];
+        v[e] = src[ic[e]];
+        for (uint32_t z = 1; z < A.nsplit; ++z) v[e] += src[z * A.sstride + ic[e]];
+        if (lane + 64u * e < hd) ss += static_cast<double>(v[e]) * static_cast<double>(v[e]);
+    }
+    float* dst = h < H ? A.q + (static_cast<uint64_t>(b) * H + h) * hd : (h == H ? A.k : A.v) + static_cast<uint64_t>(b) * hd;
+    if (h <= H) {
+        const float sc = 1.0f / sqrtf(static_cast<float>(wave_red_sum_d(ss) / static_cast<double>(hd)) + A.eps);   // :1087-1093
+#pragma unroll
+        for (uint32_t e = 0; e < 4u; ++e) x[ic[e]] = v[e] * (sc * wv[e]);   // (lanes past hd write its last value again)
+        __builtin_amdgcn_wave_barrier();   // a wave's LDS accesses complete in order
+#pragma unroll
+        for (uint32_t e = 0; e < 4u; ++e) {
+            const float a = x[ei[e]], c = x[ei[e] + half];
+            v[e] = ic[e] < half ? a * cs[e] - c * sn[e] : c * cs[e] + a * sn[e];
+        }
+    }
+#pragma unroll
+    for (uint32_t e = 0; e < 4u; ++e)
+        if (lane + 64u * e < hd) dst[lane + 64u * e] = v[e];
+}
+
 // Greedy argmax of each row's logits [n][V] (the tie rule of am_better, shaders/argmax.comp:30-43):
 // k_bd_argmax, grid (kBdArgParts, n), leaves one partial per (part, row); k_bd_argmax_final,
 // one workgroup per row, reduces them into results[b].
@@ -540,6 +599,9 @@ struct BdLayer {
     float* kc = nullptr;
     float* vc = nullptr;
     uint32_t slots = 0, G = 1, cmax = 1;
+    Kv8Dev c8{};               // over 8-bit caches
+    bool whole = false;        // attends to every position: eviction shortens it
+    float* weights = nullptr;  // [regions][max_ctx] softmax weights so far (eviction)
 };
 
 struct vrt_g3_batch {
@@ -549,6 +611,15 @@ struct vrt_g3_batch {
     std::vector<uint32_t> pos;      // next position of each sequence (host)
     std::vector<BdLayer> layers;
     std::vector<void*> allocs;
+    bool kv8 = false, evict = false;
+    std::vector<uint32_t> len;      // entries of each sequence's whole caches (evict: fewer than pos)
+    std::vector<uint32_t> region;   // where they are; with eviction, one region more than sequences:
+    uint32_t spare = 0;             //   the one that the next eviction fills
+    uint32_t* kept = nullptr;       // [max_ctx] positions an eviction kept
+    float* q8 = nullptr;            // [rows][H hd] queries, [rows][hd] keys, values for the 8-bit cache
+    float* k8 = nullptr;
+    float* v8 = nullptr;
+    void* ws8 = nullptr;            // attention workspace
     uint32_t* rows = nullptr;       // device: [3][kBdMaxRows] tokens, positions, sequences
     BdRows host_rows{};             // the same on the host, a kernel argument
     vrt_argmax_result* host_res = nullptr;   // pinned
@@ -588,12 +659,26 @@ extern "C" int vrt_g3_batch_destroy(vrt_g3_batch* B) {
     return VRT_OK;
 }
 
-extern "C" int vrt_g3_batch_create(vrt_g3* g, uint32_t max_seqs, uint32_t max_ctx, vrt_g3_batch** out) {
-    VRT_REQUIRE(g && out, "vrt_g3_batch_create: null argument");
+// A block's caches: 8-bit ones, in regions for the sequences and one to evict into.
+static int bd_layer8(vrt_g3_batch* B, BdLayer& L, uint32_t slots) {
+    const uint32_t hd = B->g->cfg.head_dim, regions = B->max_seqs + (B->evict && L.whole ? 1u : 0u);
+    L.slots = slots;
+    const Kv8Sizes z = kv8_sizes(regions, slots, 1u, hd);
+    void* p;
+    if (int rc = bd_alloc(B, z.total, &p)) return rc;
+    L.c8 = kv8_view(z, p, 1u, hd);
+    if (!B->evict || !L.whole) return VRT_OK;
+    if (int rc = bd_alloc(B, static_cast<size_t>(regions) * slots * 4u, &p)) return rc;
+    L.weights = static_cast<float*>(p);
+    return VRT_OK;
+}
+
+static int bd_create(vrt_g3* g, uint32_t max_seqs, uint32_t max_ctx, bool kv8, bool evict, const char* who, vrt_g3_batch** out) {
+    VRT_REQUIRE(g && out, "%s: null argument", who);
     *out = nullptr;
-    VRT_REQUIRE(max_seqs >= 1u && max_seqs <= kBdMaxRows, "vrt_g3_batch_create: max_seqs must be 1..%u", kBdMaxRows);
-    VRT_REQUIRE(max_ctx >= 1u && max_ctx <= g->cfg.context_length,
-                "vrt_g3_batch_create: max_ctx must be 1..context_length (%u)", g->cfg.context_length);
+    VRT_REQUIRE(max_seqs >= 1u && max_seqs <= kBdMaxRows, "%s: max_seqs must be 1..%u", who, kBdMaxRows);
+    VRT_REQUIRE(max_ctx >= 1u && max_ctx <= g->cfg.context_length, "%s: max_ctx must be 1..context_length (%u)", who,
+                g->cfg.context_length);
     const vrt_g3_config& c = g->cfg;
     const uint32_t d = c.embedding_length, H = c.head_count, hd = c.head_dim, F = c.feed_forward_length;
     const uint32_t qw = H * hd, nqkv = qw + 2u * hd;
@@ -606,6 +691,11 @@ extern "C" int vrt_g3_batch_create(vrt_g3* g, uint32_t max_seqs, uint32_t max_ct
     B->max_seqs = max_seqs;
     B->max_ctx = max_ctx;
     B->pos.assign(max_seqs, 0u);
+    B->kv8 = kv8;
+    B->evict = evict;
+    B->len.assign(max_seqs, 0u);
+    for (uint32_t i = 0; i < max_seqs; ++i) B->region.push_back(i);
+    B->spare = max_seqs;
     auto fail = [&](int rc) {
         vrt_g3_batch_destroy(B);
         return rc;
@@ -617,6 +707,11 @@ extern "C" int vrt_g3_batch_create(vrt_g3* g, uint32_t max_seqs, uint32_t max_ct
     for (size_t l = 0; l < g->layers.size(); ++l) {
         BdLayer& L = B->layers[l];
         L.slots = g->layers[l].global ? max_ctx : std::min(g->layers[l].slots, max_ctx);
+        if (kv8) {   // a window is a ring of its own size: with eviction, positions pass max_ctx
+            L.whole = g->layers[l].slots >= c.context_length;
+            if (int rc = bd_layer8(B, L, L.whole ? max_ctx : evict ? g->layers[l].slots : L.slots)) return fail(rc);
+            continue;
+        }
         const size_t kv = static_cast<size_t>(max_seqs) * L.slots * hd * 4u;
         if (int rc = bd_alloc(B, kv, &p)) return fail(rc);
         L.kc = static_cast<float*>(p);
@@ -645,8 +740,20 @@ extern "C" int vrt_g3_batch_create(vrt_g3* g, uint32_t max_seqs, uint32_t max_ct
     B->a = static_cast<_Float16*>(p);
     if (int rc = bd_alloc(B, gm_size(R, F) * 2u, &p)) return fail(rc);
     B->gg = static_cast<_Float16*>(p);
-    if (int rc = bd_alloc(B, R * gmax * (2u * H + qw) * 4u, &p)) return fail(rc);
-    B->part = static_cast<float*>(p);
+    if (kv8) {
+        if (int rc = bd_alloc(B, R * (qw + 2u * hd) * 4u, &p)) return fail(rc);
+        B->q8 = static_cast<float*>(p);
+        B->k8 = B->q8 + R * qw;
+        B->v8 = B->k8 + R * hd;
+        if (int rc = bd_alloc(B, kv8_workspace_most(R, (hd + 31u) / 32u * 32u, R, H), &B->ws8)) return fail(rc);
+        if (evict) {
+            if (int rc = bd_alloc(B, max_ctx * 4u, &p)) return fail(rc);
+            B->kept = static_cast<uint32_t*>(p);
+        }
+    } else {
+        if (int rc = bd_alloc(B, R * gmax * (2u * H + qw) * 4u, &p)) return fail(rc);
+        B->part = static_cast<float*>(p);
+    }
     if (int rc = bd_alloc(B, R * c.vocab_size * 4u, &p)) return fail(rc);
     B->logits = static_cast<float*>(p);
     if (int rc = bd_alloc(B, R * kBdArgParts * sizeof(GmBest), &p)) return fail(rc);
@@ -657,12 +764,46 @@ extern "C" int vrt_g3_batch_create(vrt_g3* g, uint32_t max_seqs, uint32_t max_ct
         if (e != hipSuccess) return fail(set_error(VRT_ERR_HIP, "hipHostMalloc failed: %s", hipGetErrorString(e)));
     }
     size_t lds = 0;
-    for (const BdLayer& L : B->layers) lds = std::max(lds, static_cast<size_t>((H + 2u) * hd + H * L.cmax) * 4u);
+    if (!kv8)
+        for (const BdLayer& L : B->layers) lds = std::max(lds, static_cast<size_t>((H + 2u) * hd + H * L.cmax) * 4u);
     if (lds > 64u * 1024u) return fail(set_error(VRT_ERR_INVALID, "batched decode: attention chunk does not fit in LDS"));
     if (int rc = gm_setup()) return fail(rc);
-    VRT_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_bd_attn), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                      static_cast<int>(lds)));
+    if (!kv8)
+        VRT_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_bd_attn), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                          static_cast<int>(lds)));
     *out = B;
+    return VRT_OK;
+}
+
+extern "C" int vrt_g3_batch_create(vrt_g3* g, uint32_t max_seqs, uint32_t max_ctx, vrt_g3_batch** out) {
+    return bd_create(g, max_seqs, max_ctx, false, false, "vrt_g3_batch_create", out);
+}
+
+extern "C" int vrt_g3_batch_create_kv8(vrt_g3* g, uint32_t max_seqs, uint32_t max_ctx, uint32_t evict, vrt_g3_batch** out) {
+    VRT_REQUIRE(evict <= 1u, "vrt_g3_batch_create_kv8: evict must be 0 or 1");
+    return bd_create(g, max_seqs, max_ctx, true, evict != 0u, "vrt_g3_batch_create_kv8", out);
+}
+
+extern "C" int vrt_g3_batch_length(vrt_g3_batch* B, uint32_t seq, uint32_t* len) {
+    VRT_REQUIRE(B && len, "vrt_g3_batch_length: null argument");
+    VRT_REQUIRE(seq < B->max_seqs, "vrt_g3_batch_length: sequence %u out of range", seq);
+    *len = B->len[seq];
+    return VRT_OK;
+}
+
+extern "C" int vrt_g3_batch_evict(vrt_g3_batch* B, uint32_t seq, uint32_t keep, uint32_t recent) {
+    VRT_REQUIRE(B, "vrt_g3_batch_evict: null batch");
+    VRT_REQUIRE(B->evict, "vrt_g3_batch_evict: the batch was not created with eviction");
+    VRT_REQUIRE(seq < B->max_seqs, "vrt_g3_batch_evict: sequence %u out of range", seq);
+    VRT_REQUIRE(keep >= 1u && keep <= B->len[seq] && recent <= keep,
+                "vrt_g3_batch_evict: needs 1 <= keep <= the sequence's length (%u), recent <= keep", B->len[seq]);
+    VRT_HIP_CHECK(hipSetDevice(B->g->ctx->device));
+    const vrt_kv8_move m = {B->region[seq], B->spare, B->len[seq], keep, recent};
+    for (const BdLayer& L : B->layers)
+        if (L.whole)   // (one buffer of kept positions: the stream orders its uses)
+            if (int rc = kv8_evict(L.c8, &m, 1u, L.weights, L.slots, B->kept, L.slots, B->g->ctx->stream)) return rc;
+    std::swap(B->region[seq], B->spare);   // a launch that failed has left the sequence as it was
+    B->len[seq] = keep;
     return VRT_OK;
 }
 
@@ -670,10 +811,11 @@ extern "C" int vrt_g3_batch_reset(vrt_g3_batch* B, uint32_t seq) {
     VRT_REQUIRE(B, "vrt_g3_batch_reset: null batch");
     if (seq == 0xffffffffu) {
         std::fill(B->pos.begin(), B->pos.end(), 0u);
+        std::fill(B->len.begin(), B->len.end(), 0u);
         return VRT_OK;
     }
     VRT_REQUIRE(seq < B->max_seqs, "vrt_g3_batch_reset: sequence %u out of range", seq);
-    B->pos[seq] = 0u;
+    B->pos[seq] = B->len[seq] = 0u;
     return VRT_OK;
 }
 
@@ -682,6 +824,37 @@ extern "C" int vrt_g3_batch_position(vrt_g3_batch* B, uint32_t seq, uint32_t* po
     VRT_REQUIRE(seq < B->max_seqs, "vrt_g3_batch_position: sequence %u out of range", seq);
     *pos = B->pos[seq];
     return VRT_OK;
+}
+
+// Block l's attention of the n rows over 8-bit caches, from the q|k|v partials to the O projection's input.
+static int bd_attend8(vrt_g3_batch* B, uint32_t l, const BdAttn& A, uint32_t n, hipStream_t s) {
+    const BdLayer& BL = B->layers[l];
+    BdQk Q{A.qkv, A.sstride, A.nsplit, A.H, A.hd, n, A.pos, A.q_norm, A.k_norm, A.cos_t, A.sin_t, A.eps, B->q8, B->k8, B->v8};
+    void* args[] = {&Q};
+    constexpr uint32_t per = kBdThreads / 64u;
+    VRT_HIP_CHECK(hipLaunchKernel(reinterpret_cast<const void*>(&k_bd_qk), dim3((A.H + 2u + per - 1u) / per, n), dim3(kBdThreads),
+                                  args, 0, s));
+    Kv8AttnArgs T{};
+    T.c = BL.c8;
+    T.o.gm = A.o;
+    T.o.gm_nkb = A.H * A.hd / 32u;
+    T.o.nonfinite = &A.st->nonfinite;
+    T.o.code = g3_code_softmax(l);
+    T.q = B->q8;
+    T.q_stride = A.H * A.hd;
+    T.w_in = T.w_out = BL.weights;
+    T.heads = T.G = A.H;
+    T.window = BL.whole ? 0u : B->g->layers[l].slots;
+    T.max_ctx = BL.slots;
+    T.scale = A.attn_scale;
+    for (uint32_t i = 0; i < n; ++i) {
+        const uint32_t q = B->host_rows.v[2][i];
+        T.s[i] = BL.whole ? Kv8Seq{B->region[q], B->len[q], 1u, 0u, i, 0u, 0u}
+                          : Kv8Seq{q, B->host_rows.v[1][i], 1u, 0u, i, 0u, 0u};
+    }
+    if (int rc = kv8_append(BL.c8, T.s, n, B->k8, B->v8, A.hd, s)) return rc;
+    const Kv8Plan P = kv8_plan(T, 1u, BL.c8.hdp, n, n, BL.weights != nullptr);
+    return kv8_attend(T, P, B->ws8, n, s);
 }
 
 // Enqueues one step over the n rows of B->host_rows.
@@ -735,7 +908,9 @@ static int bd_enqueue(vrt_g3_batch* B, uint32_t n, hipStream_t s) {
         A.o = B->a;
         A.st = B->st;
         A.block = l;
-        {
+        if (B->kv8) {
+            if (int rc = bd_attend8(B, l, A, n, s)) return rc;
+        } else {
             void* args[] = {&A};
             uint32_t nh_max = 0;   // longest history of the step's rows in this block
             for (uint32_t i = 0; i < n; ++i) nh_max = std::max(nh_max, std::min(B->host_rows.v[1][i] + 1u, BL.slots));
@@ -798,7 +973,7 @@ static int bd_enqueue(vrt_g3_batch* B, uint32_t n, hipStream_t s) {
 static int bd_fail(vrt_g3_batch* B, const uint32_t* seqs, uint32_t n, int rc, const char* msg) {
     B->last_n = 0;
     for (uint32_t i = 0; i < n; ++i)
-        if (seqs[i] < B->max_seqs) B->pos[seqs[i]] = 0u;
+        if (seqs[i] < B->max_seqs) B->pos[seqs[i]] = B->len[seqs[i]] = 0u;
     return set_error(rc, "%s", msg);
 }
 
@@ -813,7 +988,7 @@ extern "C" int vrt_g3_batch_step(vrt_g3_batch* B, const uint32_t* seqs, const ui
             VRT_REQUIRE(seqs[j] != seqs[i], "vrt_g3_batch_step: sequence %u appears twice", seqs[i]);
     }
     for (uint32_t i = 0; i < n; ++i) {
-        if (B->pos[seqs[i]] >= B->max_ctx) return set_error(VRT_ERR_STATE, "Gemma 3 context length exceeded");
+        if (B->len[seqs[i]] >= B->max_ctx || B->pos[seqs[i]] >= g->cfg.context_length) return set_error(VRT_ERR_STATE, "Gemma 3 context length exceeded");
         if (tokens[i] >= g->cfg.vocab_size)
             return bd_fail(B, seqs, n, VRT_ERR_INVALID, "Token id is outside Gemma 3 vocabulary");
     }
@@ -833,7 +1008,10 @@ extern "C" int vrt_g3_batch_step(vrt_g3_batch* B, const uint32_t* seqs, const ui
             return bd_fail(B, seqs, n, VRT_ERR_NUMERIC, "GPU argmax produced invalid result");
         results[i] = r;
     }
-    for (uint32_t i = 0; i < n; ++i) ++B->pos[seqs[i]];
+    for (uint32_t i = 0; i < n; ++i) {
+        ++B->pos[seqs[i]];
+        ++B->len[seqs[i]];
+    }
     B->last_n = n;
     return VRT_OK;
 }

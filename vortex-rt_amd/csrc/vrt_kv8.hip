@@ -5,6 +5,7 @@
 #include <cmath>
 #include <cstring>
 
+#include "vrt_gemm.hpp"
 #include "vrt_internal.hpp"
 #include "vrt_kv8.hpp"
 #include "vrt_q8_device.hpp"
@@ -207,21 +208,6 @@ __global__ void __launch_bounds__(kKvThreads) k_kv8_read(const Kv8ReadArgs A) {
 
 // ---- attention ------------------------------------------------------------------------------
 
-struct Kv8AttnArgs {
-    Kv8Dev c;
-    const float* q;
-    float* out;
-    uint64_t q_stride, out_stride;
-    float* part;          // [item][split][16 rows][hdp] unnormalised outputs, where a row tile has several splits
-    float2* part_ml;      // [item][split][16 rows]: running maximum (log2 units) and sum
-    float2* stats;        // [row][heads]: final maximum and 1 / sum (with weights)
-    const float* w_in;
-    float* w_out;
-    uint32_t heads, G, window, per, splits, max_ctx;   // per: blocks of a split
-    float scale, cap;
-    Kv8Seq s[kKvMaxSeqs];
-};
-
 // The blocks that the rows of a tile (positions pmin .. pmax) see: virtual block i is i for i < n_pre, else lo + i - n_pre.
 struct KvSpan {
     uint32_t n_pre, lo, n;
@@ -385,6 +371,31 @@ __device__ __forceinline__ bool kv_masked(const Kv8AttnArgs& A, const Kv8Seq& S,
     return !(last <= pmin && (!A.window || pmax - 32u * b < A.window));
 }
 
+// Four outputs of (row, head), and what is left to say of it.
+__device__ __forceinline__ void kv_give(const Kv8AttnArgs& A, uint32_t row, uint32_t h, uint32_t d, f4 v) {
+    const uint32_t col = h * A.c.hd + d;
+    if (!A.o.gm) {
+        *reinterpret_cast<f4*>(A.o.rows + row * A.o.stride + col) = v;
+        return;
+    }
+    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+    const uint64_t o = gm_off(row, col, A.o.gm_nkb);
+    h4 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        _Float16 a, b;
+        gm_split(v[e], a, b);
+        hi[e] = a;
+        lo[e] = b;
+    }
+    *reinterpret_cast<h4*>(A.o.gm + o) = hi;
+    *reinterpret_cast<h4*>(A.o.gm + o + kGmLo) = lo;
+}
+__device__ __forceinline__ void kv_row_done(const Kv8AttnArgs& A, uint32_t row, uint32_t h, float M, float L) {
+    if (A.stats) A.stats[static_cast<uint64_t>(row) * A.heads + h] = make_float2(M, 1.0f / L);
+    if (A.o.nonfinite && (!(L > 0.0f) || !__builtin_isfinite(L))) atomicMin(A.o.nonfinite, A.o.code);
+}
+
 // One workgroup per (split of a row tile's blocks, head, sequence); wave w takes the split's blocks w, w + 4, ...: scores on
 // the matrix cores with the tokens as rows, so that each lane holds eight weights of one query row in the order in
 // which the values are kept; running maximum and sum per row; weights times the block's value scale, as f16 pairs, times
@@ -397,7 +408,7 @@ __global__ void __launch_bounds__(kKvThreads) k_kv8_attn(const Kv8AttnArgs A) {
     const Kv8Seq& S = A.s[blockIdx.z];
     const uint32_t kvh = blockIdx.y, tile = blockIdx.x / A.splits, split = blockIdx.x - tile * A.splits;
     const uint32_t R = S.n * A.G, r0 = 16u * tile, len = S.pos + S.n;
-    if (r0 >= R) return;
+    if (r0 >= R || split >= S.splits) return;
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, m16 = lane & 15u;
     const uint32_t pmin = S.pos + r0 / A.G, pmax = S.pos + min(r0 + 15u, R - 1u) / A.G;
     const KvSpan sp = kv_span(A, S, pmin, pmax);
@@ -531,16 +542,14 @@ __global__ void __launch_bounds__(kKvThreads) k_kv8_attn(const Kv8AttnArgs A) {
     if (sp.n <= A.per) {   // the only split
         if (r >= R) return;
         const uint32_t qi = r / A.G, h = kvh * A.G + (r - qi * A.G);
-        const uint64_t row = static_cast<uint64_t>(S.row0) + qi;
 #pragma unroll
-        for (int t = 0; t < 2 * NT; ++t) {
-            const uint32_t d = 16u * t + 4u * g;
-            if (d < c.hd) *reinterpret_cast<f4*>(A.out + row * A.out_stride + h * c.hd + d) = acc[t] / L;
-        }
-        if (A.stats && g == 0u) A.stats[row * A.heads + h] = make_float2(M, 1.0f / L);
+        for (int t = 0; t < 2 * NT; ++t)
+            if (16u * t + 4u * g < c.hd) kv_give(A, S.row0 + qi, h, 16u * t + 4u * g, acc[t] / L);
+        if (g == 0u) kv_row_done(A, S.row0 + qi, h, M, L);
         return;
     }
-    const uint64_t pr = ((static_cast<uint64_t>(S.item0) + tile * c.kvh + kvh) * A.splits + split) * 16u + m16;
+    if (r >= R) return;
+    const uint64_t pr = (static_cast<uint64_t>(S.part0) + (tile * c.kvh + kvh) * S.splits + split) * 16u + m16;
 #pragma unroll
     for (int t = 0; t < 2 * NT; ++t) *reinterpret_cast<f4*>(A.part + pr * c.hdp + 16u * t + 4u * g) = acc[t];
     if (g == 0u) A.part_ml[pr] = make_float2(M, L);
@@ -555,7 +564,7 @@ __global__ void __launch_bounds__(kKvThreads) k_kv8_merge(const Kv8AttnArgs A) {
     const KvSpan sp = kv_span(A, S, S.pos + r0 / A.G, S.pos + min(r0 + 15u, R - 1u) / A.G);
     const uint32_t n = (sp.n + A.per - 1u) / A.per;
     if (n <= 1u) return;   // written by the only split
-    const uint64_t p0 = (static_cast<uint64_t>(S.item0) + tile * c.kvh + kvh) * A.splits * 16u;
+    const uint64_t p0 = (static_cast<uint64_t>(S.part0) + (tile * c.kvh + kvh) * S.splits) * 16u;
     const uint32_t hd4 = c.hd >> 2, rows = min(16u, R - r0);
     for (uint32_t u = threadIdx.x; u < rows * hd4; u += kKvThreads) {
         uint32_t rr, d;
@@ -572,9 +581,8 @@ __global__ void __launch_bounds__(kKvThreads) k_kv8_merge(const Kv8AttnArgs A) {
             o += w * *reinterpret_cast<const f4*>(A.part + (p0 + k * 16u + rr) * c.hdp + d);
         }
         const uint32_t r = r0 + rr, qi = r / A.G, h = kvh * A.G + (r - qi * A.G);
-        const uint64_t row = static_cast<uint64_t>(S.row0) + qi;
-        *reinterpret_cast<f4*>(A.out + row * A.out_stride + h * c.hd + d) = o / L;
-        if (A.stats && d == 0u) A.stats[row * A.heads + h] = make_float2(M, 1.0f / L);
+        kv_give(A, S.row0 + qi, h, d, o / L);
+        if (d == 0u) kv_row_done(A, S.row0 + qi, h, M, L);
     }
 }
 
@@ -764,45 +772,24 @@ struct OnDevice {
 
 uint64_t up256(uint64_t x) { return (x + 255u) & ~uint64_t(255); }
 
-struct Sizes {
-    uint64_t blocks, codes, scales, tail, tmax, total;
-    uint32_t nb, hdp;
-};
-
-int cache_sizes(const vrt_kv8_cache* c, const char* who, Sizes* z) {
+int check_cache(const vrt_kv8_cache* c, const char* who, Kv8Sizes* z) {
     VRT_REQUIRE(c, "%s: null cache", who);
     VRT_REQUIRE(c->max_seqs >= 1u && c->max_seqs <= 65535u, "%s: max_seqs must be 1..65535", who);
     VRT_REQUIRE(c->max_ctx >= 1u && c->max_ctx <= VRT_KV8_MAX_CTX, "%s: max_ctx must be 1..%u", who, VRT_KV8_MAX_CTX);
     VRT_REQUIRE(c->kv_heads >= 1u && c->kv_heads <= 1024u, "%s: kv_heads must be 1..1024", who);
     VRT_REQUIRE(c->head_dim >= 4u && c->head_dim <= 256u && c->head_dim % 4u == 0u,
                 "%s: head_dim must be a multiple of 4, 4..256", who);
-    z->nb = (c->max_ctx + kKvBlock - 1u) / kKvBlock;
-    z->hdp = (c->head_dim + 31u) / 32u * 32u;
-    const uint64_t heads = static_cast<uint64_t>(c->max_seqs) * c->kv_heads;
-    z->blocks = heads * z->nb;   // below 2^47
-    z->codes = up256(z->blocks * 64u * z->hdp);
-    z->scales = up256(z->blocks * sizeof(float2));
-    z->tail = up256(heads * 128u * z->hdp * 4u);
-    z->tmax = up256(heads * 128u * 4u);
-    z->total = z->codes + z->scales + z->tail + z->tmax;
+    *z = kv8_sizes(c->max_seqs, c->max_ctx, c->kv_heads, c->head_dim);
     return VRT_OK;
 }
 
 int cache_view(const vrt_kv8_cache* c, const char* who, Kv8Dev* d) {
-    Sizes z;
-    if (int rc = cache_sizes(c, who, &z)) return rc;
+    Kv8Sizes z;
+    if (int rc = check_cache(c, who, &z)) return rc;
     VRT_REQUIRE(c->data && (reinterpret_cast<uintptr_t>(c->data) & 255u) == 0u, "%s: cache memory must be 256-byte aligned", who);
     VRT_REQUIRE(c->bytes >= z.total, "%s: cache memory is too small (%llu of %llu bytes)", who,
                 static_cast<unsigned long long>(c->bytes), static_cast<unsigned long long>(z.total));
-    auto* p = static_cast<uint8_t*>(c->data);
-    d->codes = p;
-    d->scales = reinterpret_cast<float2*>(p + z.codes);
-    d->tail = reinterpret_cast<float*>(p + z.codes + z.scales);
-    d->tmax = reinterpret_cast<float*>(p + z.codes + z.scales + z.tail);
-    d->nb = z.nb;
-    d->kvh = c->kv_heads;
-    d->hd = c->head_dim;
-    d->hdp = z.hdp;
+    *d = kv8_view(z, c->data, c->kv_heads, c->head_dim);
     return VRT_OK;
 }
 
@@ -815,7 +802,7 @@ int check_rows(const vrt_kv8_cache* c, const vrt_kv8_rows* rows, uint32_t n, con
         VRT_REQUIRE(r.seq < c->max_seqs, "%s: sequence %u out of range", who, r.seq);
         for (uint32_t j = 0; j < i; ++j) VRT_REQUIRE(rows[j].seq != r.seq, "%s: sequence %u appears twice", who, r.seq);
         VRT_REQUIRE(r.pos <= VRT_KV8_MAX_CTX && r.n <= VRT_KV8_MAX_CTX - r.pos, "%s: positions past %u", who, VRT_KV8_MAX_CTX);
-        s[i] = Kv8Seq{r.seq, r.pos, r.n, r.prefix, static_cast<uint32_t>(row), 0u};
+        s[i] = Kv8Seq{r.seq, r.pos, r.n, r.prefix, static_cast<uint32_t>(row), 0u, 0u};
         row += r.n;
     }
     VRT_REQUIRE(row <= 0x7fffffffu, "%s: too many rows", who);
@@ -835,66 +822,44 @@ int check_array(const void* p, uint64_t* stride, uint64_t width, const char* who
 // Blocks that a span of positions touches.
 uint32_t touched(const Kv8Seq& s) { return s.n ? ((s.pos + s.n - 1u) >> 5) - (s.pos >> 5) + 1u : 0u; }
 
-struct AttnPlan {
-    Kv8AttnArgs A;
-    uint32_t tiles, max_blocks;
-    uint64_t rows, items, part, ml, stats, total;
-};
+// The most blocks that a row tile of a sequence sees.
+uint32_t most_blocks(const Kv8Seq& s, uint32_t window) {
+    const uint32_t len = s.pos + s.n, pre = std::min(s.prefix, len), all = (len + 31u) / 32u;
+    if (!window) return all;
+    // a tile's rows span 16 positions at most
+    const uint64_t w = static_cast<uint64_t>((pre + 31u) / 32u) + (static_cast<uint64_t>(window) + 15u + 31u) / 32u + 1u;
+    return static_cast<uint32_t>(std::min<uint64_t>(all, w));
+}
 
 int attn_plan(const vrt_kv8_cache* c, const vrt_kv8_attn* at, const vrt_kv8_rows* rows, uint32_t n, bool scored, const char* who,
-              AttnPlan* P) {
-    Sizes z;
-    if (int rc = cache_sizes(c, who, &z)) return rc;
+              Kv8AttnArgs& A, Kv8Plan* P, uint64_t* total) {
+    Kv8Sizes z;
+    if (int rc = check_cache(c, who, &z)) return rc;
     VRT_REQUIRE(at, "%s: null attention", who);
     VRT_REQUIRE(at->heads >= 1u && at->heads <= 65535u && at->heads % c->kv_heads == 0u,
                 "%s: heads must be a multiple of kv_heads, at most 65535", who);
     VRT_REQUIRE(std::isfinite(at->scale), "%s: scale is not finite", who);
     VRT_REQUIRE(std::isfinite(at->softcap) && at->softcap >= 0.0f, "%s: softcap must be finite, not negative", who);
-    Kv8AttnArgs& A = P->A;
-    if (int rc = check_rows(c, rows, n, who, A.s, &P->rows)) return rc;
+    if (int rc = check_rows(c, rows, n, who, A.s, total)) return rc;
     A.heads = at->heads;
     A.G = at->heads / c->kv_heads;
     A.window = at->window;
     A.scale = at->scale;
     A.cap = at->softcap;
     A.max_ctx = c->max_ctx;
-    P->tiles = 0;
-    P->max_blocks = 0;
-    P->items = 0;
-    uint64_t blocks = 0;   // of all row tiles and heads
+    uint64_t items = 0;
     for (uint32_t i = 0; i < n; ++i) {
-        Kv8Seq& s = A.s[i];
+        const Kv8Seq& s = A.s[i];
         if (s.n == 0u) continue;
         const uint32_t len = s.pos + s.n, pre = std::min(s.prefix, len);
-        const uint32_t first = A.window && s.pos + 1u > A.window ? s.pos + 1u - A.window : 0u;   // of the first query
-        const uint32_t seen = pre ? 0u : first >> 5;
-        VRT_REQUIRE(static_cast<uint64_t>(seen) + z.nb >= len / kKvBlock, "%s: sequence %u: the cache no longer holds position %u", who,
-                    s.seq, pre ? 0u : first);
+        const uint32_t first = pre ? 0u : A.window && s.pos + 1u > A.window ? s.pos + 1u - A.window : 0u;   // that a query sees
+        VRT_REQUIRE(static_cast<uint64_t>(first >> 5) + z.nb >= len / kKvBlock, "%s: sequence %u: the cache no longer holds position %u",
+                    who, s.seq, first);
         VRT_REQUIRE(!scored || len <= c->max_ctx, "%s: weights need pos + n <= max_ctx", who);
-        VRT_REQUIRE(static_cast<uint64_t>(s.n) * A.G <= 0x3fffffffu, "%s: too many rows", who);
-        const uint32_t tiles = (s.n * A.G + 15u) / 16u;
-        uint32_t nb = (len + 31u) / 32u;
-        if (A.window) {   // a tile's rows span 16 positions at most
-            const uint64_t w = static_cast<uint64_t>((pre + 31u) / 32u) + (static_cast<uint64_t>(A.window) + 15u + 31u) / 32u + 1u;
-            nb = static_cast<uint32_t>(std::min<uint64_t>(nb, w));
-        }
-        s.item0 = static_cast<uint32_t>(P->items);
-        P->items += static_cast<uint64_t>(tiles) * c->kv_heads;
-        VRT_REQUIRE(P->items <= 0x7fffffffu, "%s: too many rows", who);
-        blocks += static_cast<uint64_t>(tiles) * c->kv_heads * nb;
-        P->tiles = std::max(P->tiles, tiles);
-        P->max_blocks = std::max(P->max_blocks, nb);
+        items += (static_cast<uint64_t>(s.n) * A.G + 15u) / 16u * c->kv_heads;
     }
-    // about 1024 workgroups, of four blocks at least
-    A.per = static_cast<uint32_t>(std::max<uint64_t>(4u, (blocks + 1023u) / 1024u));
-    A.per = (A.per + 3u) & ~3u;
-    A.splits = P->max_blocks ? (P->max_blocks + A.per - 1u) / A.per : 1u;
-    VRT_REQUIRE(static_cast<uint64_t>(P->tiles) * A.splits <= 0x7fffffffu, "%s: too many rows", who);
-    const uint64_t prows = A.splits > 1u ? P->items * A.splits * 16u : 0u;
-    P->part = up256(prows * z.hdp * 4u);
-    P->ml = up256(prows * sizeof(float2));
-    P->stats = scored ? up256(P->rows * A.heads * sizeof(float2)) : 0u;
-    P->total = P->part + P->ml + P->stats;
+    VRT_REQUIRE(*total * A.G <= 0x3fffffffu && items <= 0x3fffffffu, "%s: too many rows", who);
+    *P = kv8_plan(A, c->kv_heads, z.hdp, n, *total, scored);
     return VRT_OK;
 }
 
@@ -933,14 +898,127 @@ int launch(const void* fn, dim3 grid, uint32_t threads, Args& A, hipStream_t s) 
 }
 
 }  // namespace
+
+Kv8Sizes kv8_sizes(uint32_t max_seqs, uint32_t max_ctx, uint32_t kv_heads, uint32_t head_dim) {
+    Kv8Sizes z;
+    z.nb = (max_ctx + kKvBlock - 1u) / kKvBlock;
+    z.hdp = (head_dim + 31u) / 32u * 32u;
+    const uint64_t heads = static_cast<uint64_t>(max_seqs) * kv_heads, blocks = heads * z.nb;   // below 2^47
+    z.codes = up256(blocks * 64u * z.hdp);
+    z.scales = up256(blocks * sizeof(float2));
+    z.tail = up256(heads * 128u * z.hdp * 4u);
+    z.tmax = up256(heads * 128u * 4u);
+    z.total = z.codes + z.scales + z.tail + z.tmax;
+    return z;
+}
+
+Kv8Dev kv8_view(const Kv8Sizes& z, void* data, uint32_t kv_heads, uint32_t head_dim) {
+    auto* p = static_cast<uint8_t*>(data);
+    Kv8Dev d;
+    d.codes = p;
+    d.scales = reinterpret_cast<float2*>(p + z.codes);
+    d.tail = reinterpret_cast<float*>(p + z.codes + z.scales);
+    d.tmax = reinterpret_cast<float*>(p + z.codes + z.scales + z.tail);
+    d.nb = z.nb;
+    d.kvh = kv_heads;
+    d.hd = head_dim;
+    d.hdp = z.hdp;
+    return d;
+}
+
+// About kKvSplits workgroups, of four blocks at least.
+constexpr uint64_t kKvSplits = 1024;
+
+Kv8Plan kv8_plan(Kv8AttnArgs& A, uint32_t kvh, uint32_t hdp, uint32_t n, uint64_t rows, bool scored) {
+    Kv8Plan P{};
+    uint64_t blocks = 0;   // of all row tiles and heads
+    for (uint32_t i = 0; i < n; ++i)
+        blocks += static_cast<uint64_t>((A.s[i].n * A.G + 15u) / 16u) * kvh * most_blocks(A.s[i], A.window);
+    const uint64_t per = std::max<uint64_t>(4u, (blocks + kKvSplits - 1u) / kKvSplits);
+    A.per = static_cast<uint32_t>((per + 3u) & ~3ull);
+    A.splits = 1u;
+    uint64_t place = 0;
+    for (uint32_t i = 0; i < n; ++i) {
+        Kv8Seq& s = A.s[i];
+        const uint32_t tiles = (s.n * A.G + 15u) / 16u;
+        s.splits = std::max(1u, (most_blocks(s, A.window) + A.per - 1u) / A.per);
+        s.part0 = static_cast<uint32_t>(place);
+        if (s.splits > 1u) place += static_cast<uint64_t>(tiles) * kvh * s.splits;
+        A.splits = std::max(A.splits, s.splits);
+        P.tiles = std::max(P.tiles, tiles);
+    }
+    P.part = up256(place * 16u * hdp * 4u);
+    P.ml = up256(place * 16u * sizeof(float2));
+    P.stats = scored ? up256(rows * A.heads * sizeof(float2)) : 0u;
+    P.total = P.part + P.ml + P.stats;
+    return P;
+}
+
+// (a sequence's splits are at most its blocks / per + 1, and all blocks / per at most kKvSplits)
+uint64_t kv8_workspace_most(uint64_t items, uint32_t hdp, uint64_t rows, uint32_t heads) {
+    const uint64_t place = kKvSplits + items;
+    return up256(place * 16u * hdp * 4u) + up256(place * 16u * sizeof(float2)) + up256(rows * heads * sizeof(float2));
+}
+
+int kv8_append(const Kv8Dev& c, const Kv8Seq* seqs, uint32_t n, const float* k, const float* v, uint64_t stride, hipStream_t s) {
+    Kv8AppendArgs A{};
+    A.c = c;
+    A.x[0] = k;
+    A.x[1] = v;
+    A.stride = stride;
+    uint32_t blocks = 0;
+    for (uint32_t i = 0; i < n; ++i) {
+        A.s[i] = seqs[i];
+        blocks = std::max(blocks, touched(seqs[i]));
+    }
+    if (blocks == 0u) return VRT_OK;
+    return launch(reinterpret_cast<const void*>(&k_kv8_append), dim3(blocks, 2u * c.kvh, n), kKvThreads, A, s);
+}
+
+int kv8_attend(Kv8AttnArgs& A, const Kv8Plan& P, void* workspace, uint32_t n, hipStream_t s) {
+    auto* ws = static_cast<uint8_t*>(workspace);
+    A.part = reinterpret_cast<float*>(ws);
+    A.part_ml = reinterpret_cast<float2*>(ws + P.part);
+    A.stats = A.w_out ? reinterpret_cast<float2*>(ws + P.part + P.ml) : nullptr;
+    const uint32_t nt = A.c.hdp / 32u;
+    const bool cap = A.cap > 0.0f;
+    if (int rc = launch(cap ? attn_kernel<true>(nt) : attn_kernel<false>(nt), dim3(P.tiles * A.splits, A.c.kvh, n), kKvThreads, A, s))
+        return rc;
+    if (A.splits > 1u)
+        if (int rc = launch(reinterpret_cast<const void*>(&k_kv8_merge), dim3(P.tiles, A.c.kvh, n), kKvThreads, A, s)) return rc;
+    if (!A.w_out) return VRT_OK;
+    uint32_t len = 0;
+    for (uint32_t i = 0; i < n; ++i)
+        if (A.s[i].n) len = std::max(len, A.s[i].pos + A.s[i].n);
+    return launch(cap ? weights_kernel<true>(nt) : weights_kernel<false>(nt), dim3((len + 127u) / 128u, A.c.kvh, n), kKvThreads, A, s);
+}
+
+int kv8_evict(const Kv8Dev& c, const vrt_kv8_move* moves, uint32_t n, float* weights, uint32_t max_ctx, uint32_t* kept,
+              uint64_t kept_stride, hipStream_t s) {
+    Kv8EvictArgs A{};
+    A.c = c;
+    A.w = weights;
+    A.kept = kept;
+    A.kept_stride = kept_stride;
+    A.max_ctx = max_ctx;
+    uint32_t keep = 0;
+    for (uint32_t i = 0; i < n; ++i) {
+        A.m[i] = moves[i];
+        keep = std::max(keep, moves[i].keep);
+    }
+    if (keep == 0u) return VRT_OK;
+    if (int rc = launch(reinterpret_cast<const void*>(&k_kv8_select), dim3(c.kvh, n), kKvSelThreads, A, s)) return rc;
+    return launch(reinterpret_cast<const void*>(&k_kv8_gather), dim3((keep + 31u) / 32u, 2u * c.kvh, n), kKvThreads, A, s);
+}
+
 }  // namespace vrt
 
 using namespace vrt;
 
 extern "C" int vrt_kv8_cache_bytes(const vrt_kv8_cache* cache, uint64_t* bytes) {
     VRT_REQUIRE(bytes, "vrt_kv8_cache_bytes: null argument");
-    Sizes z;
-    if (int rc = cache_sizes(cache, "vrt_kv8_cache_bytes", &z)) return rc;
+    Kv8Sizes z;
+    if (int rc = check_cache(cache, "vrt_kv8_cache_bytes", &z)) return rc;
     *bytes = z.total;
     return VRT_OK;
 }
@@ -949,25 +1027,21 @@ extern "C" int vrt_kv8_append(vrt_ctx* ctx, const vrt_kv8_cache* cache, const vr
                               const float* k, const float* v, uint64_t kv_stride) {
     const char* who = "vrt_kv8_append";
     VRT_REQUIRE(ctx, "%s: null context", who);
-    Kv8AppendArgs A{};
-    if (int rc = cache_view(cache, who, &A.c)) return rc;
+    Kv8Dev c;
+    Kv8Seq s[kKvMaxSeqs];
     uint64_t total;
-    if (int rc = check_rows(cache, rows, n_seqs, who, A.s, &total)) return rc;
-    A.stride = kv_stride;
-    if (int rc = check_array(k, &A.stride, static_cast<uint64_t>(cache->kv_heads) * cache->head_dim, who, "k")) return rc;
-    if (int rc = check_array(v, &A.stride, static_cast<uint64_t>(cache->kv_heads) * cache->head_dim, who, "v")) return rc;
-    A.x[0] = k;
-    A.x[1] = v;
-    uint32_t blocks = 0;
-    for (uint32_t i = 0; i < n_seqs; ++i) {
-        const uint32_t t = touched(A.s[i]);
-        VRT_REQUIRE(t <= A.c.nb, "%s: sequence %u: more blocks than a region of %u positions holds", who, A.s[i].seq, cache->max_ctx);
-        blocks = std::max(blocks, t);
-    }
-    if (blocks == 0u) return VRT_OK;
+    if (int rc = cache_view(cache, who, &c)) return rc;
+    if (int rc = check_rows(cache, rows, n_seqs, who, s, &total)) return rc;
+    const uint64_t width = static_cast<uint64_t>(cache->kv_heads) * cache->head_dim;
+    if (int rc = check_array(k, &kv_stride, width, who, "k")) return rc;
+    if (int rc = check_array(v, &kv_stride, width, who, "v")) return rc;
+    for (uint32_t i = 0; i < n_seqs; ++i)
+        VRT_REQUIRE(touched(s[i]) <= c.nb, "%s: sequence %u: more blocks than a region of %u positions holds", who, s[i].seq,
+                    cache->max_ctx);
+    if (total == 0u) return VRT_OK;
     OnDevice on(ctx->device);
     VRT_HIP_CHECK(on.err);
-    return launch(reinterpret_cast<const void*>(&k_kv8_append), dim3(blocks, 2u * A.c.kvh, n_seqs), kKvThreads, A, ctx->stream);
+    return kv8_append(c, s, n_seqs, k, v, kv_stride, ctx->stream);
 }
 
 extern "C" int vrt_kv8_read(vrt_ctx* ctx, const vrt_kv8_cache* cache, const vrt_kv8_rows* rows, uint32_t n_seqs,
@@ -979,8 +1053,9 @@ extern "C" int vrt_kv8_read(vrt_ctx* ctx, const vrt_kv8_cache* cache, const vrt_
     uint64_t total;
     if (int rc = check_rows(cache, rows, n_seqs, who, A.s, &total)) return rc;
     A.stride = kv_stride;
-    if (int rc = check_array(k, &A.stride, static_cast<uint64_t>(cache->kv_heads) * cache->head_dim, who, "k")) return rc;
-    if (int rc = check_array(v, &A.stride, static_cast<uint64_t>(cache->kv_heads) * cache->head_dim, who, "v")) return rc;
+    const uint64_t width = static_cast<uint64_t>(cache->kv_heads) * cache->head_dim;
+    if (int rc = check_array(k, &A.stride, width, who, "k")) return rc;
+    if (int rc = check_array(v, &A.stride, width, who, "v")) return rc;
     A.x[0] = k;
     A.x[1] = v;
     uint32_t blocks = 0;
@@ -1003,8 +1078,10 @@ extern "C" int vrt_kv8_attend_workspace(const vrt_kv8_cache* cache, const vrt_kv
                                         uint32_t n_seqs, uint32_t scored, uint64_t* bytes) {
     const char* who = "vrt_kv8_attend_workspace";
     VRT_REQUIRE(bytes, "%s: null argument", who);
-    AttnPlan P{};
-    if (int rc = attn_plan(cache, attn, rows, n_seqs, scored != 0u, who, &P)) return rc;
+    Kv8AttnArgs A{};
+    Kv8Plan P{};
+    uint64_t total;
+    if (int rc = attn_plan(cache, attn, rows, n_seqs, scored != 0u, who, A, &P, &total)) return rc;
     *bytes = P.total;
     return VRT_OK;
 }
@@ -1014,59 +1091,41 @@ extern "C" int vrt_kv8_attend(vrt_ctx* ctx, const vrt_kv8_cache* cache, const vr
                               const float* weights_in, float* weights_out, void* workspace, uint64_t workspace_bytes) {
     const char* who = "vrt_kv8_attend";
     VRT_REQUIRE(ctx, "%s: null context", who);
-    AttnPlan P{};
-    if (int rc = attn_plan(cache, attn, rows, n_seqs, weights_out != nullptr, who, &P)) return rc;
-    Kv8AttnArgs& A = P.A;
+    Kv8AttnArgs A{};
+    Kv8Plan P{};
+    uint64_t total;
+    if (int rc = attn_plan(cache, attn, rows, n_seqs, weights_out != nullptr, who, A, &P, &total)) return rc;
     if (int rc = cache_view(cache, who, &A.c)) return rc;
-    A.q_stride = q_stride;
-    A.out_stride = out_stride;
     const uint64_t width = static_cast<uint64_t>(A.heads) * cache->head_dim;
-    if (int rc = check_array(q, &A.q_stride, width, who, "q")) return rc;
-    if (int rc = check_array(out, &A.out_stride, width, who, "out")) return rc;
+    if (int rc = check_array(q, &q_stride, width, who, "q")) return rc;
+    if (int rc = check_array(out, &out_stride, width, who, "out")) return rc;
     VRT_REQUIRE(weights_out || !weights_in, "%s: weights_in without weights_out", who);
     VRT_REQUIRE(((reinterpret_cast<uintptr_t>(weights_in) | reinterpret_cast<uintptr_t>(weights_out)) & 3u) == 0u,
                 "%s: weights must be 4-byte aligned", who);
     VRT_REQUIRE(P.total == 0u || (workspace && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0u && workspace_bytes >= P.total),
                 "%s: workspace must be 256-byte aligned, at least %llu bytes", who, static_cast<unsigned long long>(P.total));
-    if (P.rows == 0u) return VRT_OK;
+    if (total == 0u) return VRT_OK;
     A.q = q;
-    A.out = out;
+    A.q_stride = q_stride;
+    A.o.rows = out;
+    A.o.stride = out_stride;
     A.w_in = weights_in;
     A.w_out = weights_out;
-    auto* ws = static_cast<uint8_t*>(workspace);
-    A.part = reinterpret_cast<float*>(ws);
-    A.part_ml = reinterpret_cast<float2*>(ws + P.part);
-    A.stats = weights_out ? reinterpret_cast<float2*>(ws + P.part + P.ml) : nullptr;
     OnDevice on(ctx->device);
     VRT_HIP_CHECK(on.err);
-    const uint32_t nt = A.c.hdp / 32u;
-    const bool cap = A.cap > 0.0f;
-    if (int rc = launch(cap ? attn_kernel<true>(nt) : attn_kernel<false>(nt), dim3(P.tiles * A.splits, A.c.kvh, n_seqs), kKvThreads, A,
-                        ctx->stream))
-        return rc;
-    if (A.splits > 1u)
-        if (int rc = launch(reinterpret_cast<const void*>(&k_kv8_merge), dim3(P.tiles, A.c.kvh, n_seqs), kKvThreads, A, ctx->stream))
-            return rc;
-    if (weights_out) {
-        uint32_t len = 0;
-        for (uint32_t i = 0; i < n_seqs; ++i)
-            if (A.s[i].n) len = std::max(len, A.s[i].pos + A.s[i].n);
-        return launch(cap ? weights_kernel<true>(nt) : weights_kernel<false>(nt), dim3((len + 127u) / 128u, A.c.kvh, n_seqs), kKvThreads,
-                      A, ctx->stream);
-    }
-    return VRT_OK;
+    return kv8_attend(A, P, workspace, n_seqs, ctx->stream);
 }
 
 extern "C" int vrt_kv8_evict(vrt_ctx* ctx, const vrt_kv8_cache* cache, const vrt_kv8_move* moves, uint32_t n, float* weights,
                              uint32_t* kept, uint64_t kept_stride) {
     const char* who = "vrt_kv8_evict";
     VRT_REQUIRE(ctx && moves && weights && kept, "%s: null argument", who);
-    Kv8EvictArgs A{};
-    if (int rc = cache_view(cache, who, &A.c)) return rc;
+    Kv8Dev c;
+    if (int rc = cache_view(cache, who, &c)) return rc;
     VRT_REQUIRE(n >= 1u && n <= kKvMaxSeqs, "%s: n must be 1..%u", who, kKvMaxSeqs);
     VRT_REQUIRE(((reinterpret_cast<uintptr_t>(weights) | reinterpret_cast<uintptr_t>(kept)) & 3u) == 0u,
                 "%s: weights and kept must be 4-byte aligned", who);
-    uint32_t keep = 0;
+    VRT_REQUIRE(kept_stride <= (1ull << 32), "%s: kept_stride is too large", who);
     for (uint32_t i = 0; i < n; ++i) {
         const vrt_kv8_move& m = moves[i];
         VRT_REQUIRE(m.src < cache->max_seqs && m.dst < cache->max_seqs, "%s: sequence out of range", who);
@@ -1076,17 +1135,8 @@ extern "C" int vrt_kv8_evict(vrt_ctx* ctx, const vrt_kv8_cache* cache, const vrt
             VRT_REQUIRE(moves[j].src != m.dst, "%s: sequence %u is a source and a destination", who, m.dst);
             VRT_REQUIRE(j == i || moves[j].dst != m.dst, "%s: sequence %u is a destination twice", who, m.dst);
         }
-        A.m[i] = m;
-        keep = std::max(keep, m.keep);
     }
-    VRT_REQUIRE(kept_stride <= (1ull << 32), "%s: kept_stride is too large", who);
-    if (keep == 0u) return VRT_OK;
-    A.w = weights;
-    A.kept = kept;
-    A.kept_stride = kept_stride;
-    A.max_ctx = cache->max_ctx;
     OnDevice on(ctx->device);
     VRT_HIP_CHECK(on.err);
-    if (int rc = launch(reinterpret_cast<const void*>(&k_kv8_select), dim3(A.c.kvh, n), kKvSelThreads, A, ctx->stream)) return rc;
-    return launch(reinterpret_cast<const void*>(&k_kv8_gather), dim3((keep + 31u) / 32u, 2u * A.c.kvh, n), kKvThreads, A, ctx->stream);
+    return kv8_evict(c, moves, n, weights, cache->max_ctx, kept, kept_stride, ctx->stream);
 }

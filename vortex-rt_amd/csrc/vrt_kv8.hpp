@@ -39,7 +39,54 @@ struct Kv8Dev {
 struct Kv8Seq {
     uint32_t seq, pos, n, prefix;   // as vrt_kv8_rows
     uint32_t row0;                  // its first row of q / k / v / out
-    uint32_t item0;                 // its first (row tile, head) of the attention's workspace
+    uint32_t splits;                // splits of each of its (row tile, head)s, and the first's place in the workspace
+    uint32_t part0;
 };
+
+// Attention outputs: fp32 rows, or (gm not null) the activation buffer of a projection (vrt_gemm.hpp).
+struct Kv8Out {
+    float* rows;
+    uint64_t stride;
+    _Float16* gm;
+    uint32_t gm_nkb;
+    uint32_t* nonfinite;   // not null: a row whose sum of weights is not a positive number lowers it to code
+    uint32_t code;
+};
+
+struct Kv8AttnArgs {
+    Kv8Dev c;
+    Kv8Out o;
+    const float* q;
+    uint64_t q_stride;
+    float* part;          // [place][16 rows][hdp] unnormalised outputs, where a row tile has several splits
+    float2* part_ml;      // [place][16 rows]: running maximum (log2 units) and sum
+    float2* stats;        // [row][heads]: final maximum and 1 / sum (with weights)
+    const float* w_in;
+    float* w_out;
+    uint32_t heads, G, window, per, splits, max_ctx;   // per: blocks of a split; splits: the most of a sequence
+    float scale, cap;
+    Kv8Seq s[kKvMaxSeqs];
+};
+
+// A cache's memory: sizes of its parts, and the view of it.
+struct Kv8Sizes {
+    uint64_t codes, scales, tail, tmax, total;
+    uint32_t nb, hdp;
+};
+Kv8Sizes kv8_sizes(uint32_t max_seqs, uint32_t max_ctx, uint32_t kv_heads, uint32_t head_dim);
+Kv8Dev kv8_view(const Kv8Sizes& z, void* data, uint32_t kv_heads, uint32_t head_dim);
+
+// Launches on checked arguments. kv8_plan fills the split of A (heads, G, window and s[].seq .. row0 given) and says what the
+// workspace has to hold: at most kv8_workspace_most(items, ...) bytes, items the (row tile, head)s of the call.
+struct Kv8Plan {
+    uint32_t tiles;   // the most of a sequence
+    uint64_t part, ml, stats, total;
+};
+Kv8Plan kv8_plan(Kv8AttnArgs& A, uint32_t kvh, uint32_t hdp, uint32_t n, uint64_t rows, bool scored);
+uint64_t kv8_workspace_most(uint64_t items, uint32_t hdp, uint64_t rows, uint32_t heads);
+int kv8_append(const Kv8Dev& c, const Kv8Seq* seqs, uint32_t n, const float* k, const float* v, uint64_t stride, hipStream_t s);
+int kv8_attend(Kv8AttnArgs& A, const Kv8Plan& P, void* workspace, uint32_t n, hipStream_t s);
+int kv8_evict(const Kv8Dev& c, const vrt_kv8_move* moves, uint32_t n, float* weights, uint32_t max_ctx, uint32_t* kept,
+              uint64_t kept_stride, hipStream_t s);
 
 }  // namespace vrt

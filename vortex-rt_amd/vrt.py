@@ -126,6 +126,9 @@ SIGNATURES = {
     "vrt_g3_read_trace": (_I, [_P, _P, _U64, C.POINTER(_U32), C.POINTER(_U32)]),
     "vrt_g3_read_exchange": (_I, [_P, _U32, _P, _U64, C.POINTER(_U64)]),
     "vrt_g3_batch_create": (_I, [_P, _U32, _U32, C.POINTER(_P)]),
+    "vrt_g3_batch_create_kv8": (_I, [_P, _U32, _U32, _U32, C.POINTER(_P)]),
+    "vrt_g3_batch_evict": (_I, [_P, _U32, _U32, _U32]),
+    "vrt_g3_batch_length": (_I, [_P, _U32, C.POINTER(_U32)]),
     "vrt_g3_batch_destroy": (_I, [_P]),
     "vrt_g3_batch_reset": (_I, [_P, _U32]),
     "vrt_g3_batch_step": (_I, [_P, _P, _P, _U32, _P]),
@@ -630,15 +633,22 @@ class Gemma3:
 
 class Gemma3Batch:
     """Batched greedy decode over independent sequences that share a Gemma3 executor's weights
-    (vrt_g3_batch_*): each sequence has its own KV cache and position."""
+    (vrt_g3_batch_*): each sequence has its own KV cache and position. kv: cache entries "f32" or "i8"
+    (8-bit, vrt_kv8_*); evict: with "i8", sequences' caches can be shortened (evict())."""
 
-    def __init__(self, model: "Gemma3", max_seqs: int, max_ctx: int):
+    def __init__(self, model: "Gemma3", max_seqs: int, max_ctx: int, kv: str = "f32", evict: bool = False):
         self.h = None
+        if kv not in ("f32", "i8") or (evict and kv != "i8"):
+            raise ValueError(f"no batch with {kv!r} entries{' and eviction' if evict else ''}")
         self.model = model
         self.max_seqs = max_seqs
         h = C.c_void_p()
-        check(lib().vrt_g3_batch_create(model.h, max_seqs, max_ctx, C.byref(h)))
+        if kv == "i8":
+            check(lib().vrt_g3_batch_create_kv8(model.h, max_seqs, max_ctx, int(evict), C.byref(h)))
+        else:
+            check(lib().vrt_g3_batch_create(model.h, max_seqs, max_ctx, C.byref(h)))
         self.h = h.value
+        self.max_ctx = max_ctx
         model._batches.add(self)
 
     def close(self):
@@ -657,6 +667,17 @@ class Gemma3Batch:
         check(lib().vrt_g3_batch_position(self.h, seq, C.byref(p)))
         return p.value
 
+    def length(self, seq: int) -> int:
+        """Entries of the sequence's caches (its position, or fewer after an eviction)."""
+        n = C.c_uint32()
+        check(lib().vrt_g3_batch_length(self.h, seq, C.byref(n)))
+        return n.value
+
+    def evict(self, seq: int, keep: int, recent: int):
+        """Of the sequence's cache entries the last `recent` stay and those of the others that attention weighed most,
+        `keep` in all."""
+        check(lib().vrt_g3_batch_evict(self.h, seq, keep, recent))
+
     def step(self, seqs, tokens):
         """One step: sequence seqs[i] consumes tokens[i]; returns (indices, values)."""
         s = np.ascontiguousarray(seqs, dtype=np.uint32)
@@ -672,10 +693,10 @@ class Gemma3Batch:
         check(lib().vrt_g3_batch_logits(self.h, row, ptr(out), out.size))
         return out
 
-    def generate(self, prompts, max_new: int, starts=None, eos=None):
+    def generate(self, prompts, max_new: int, starts=None, eos=None, evict=None):
         """Continuous batching: sequence i joins at step starts[i] (default 0), feeds its prompt
         one token per step, then its own greedy tokens, until max_new tokens or EOS. Returns the
-        generated ids per sequence."""
+        generated ids per sequence. evict = (keep, recent): a sequence whose caches are full is shortened so."""
         n = len(prompts)
         if n > self.max_seqs:
             raise ValueError("more prompts than sequences")
@@ -689,6 +710,10 @@ class Gemma3Batch:
         while not all(done):
             rows = [i for i in range(n) if not done[i] and step >= starts[i]]
             if rows:
+                if evict is not None:
+                    for i in rows:
+                        if self.length(i) >= self.max_ctx:
+                            self.evict(i, *evict)
                 toks = [feed[i][0] if feed[i] else gen[i][-1] for i in rows]
                 idx, _ = self.step(rows, toks)
                 for i, r in zip(rows, idx):
