@@ -58,11 +58,12 @@ def test_cache_sizes(kw, match):
 
 
 def test_cache_bytes():
-    """Two regions, three heads, 70 positions (3 blocks), 40 dims in 64: codes, scales, the fp32 rows of two blocks and their maxima."""
+    """Two regions, three heads, 70 positions (3 blocks), 40 dims in 64: codes, scales, two blocks' rows in fp32, in pairs of
+    halves, and the rows' factors."""
     n = C.c_uint64()
     vrt.check(vrt.lib().vrt_kv8_cache_bytes(C.byref(_cache(max_seqs=2, kv_heads=3, max_ctx=70, head_dim=40)), C.byref(n)))
     up = lambda x: (x + 255) // 256 * 256  # noqa: E731
-    assert n.value == up(2 * 3 * 3 * 64 * 64) + up(2 * 3 * 3 * 8) + up(2 * 3 * 128 * 64 * 4) + up(2 * 3 * 128 * 4)
+    assert n.value == up(2 * 3 * 3 * 64 * 64) + up(2 * 3 * 3 * 8) + up(2 * 3 * 128 * 64 * 4) + up(2 * 3 * 128 * 64 * 4) + up(2 * 3 * 128 * 4)
 
 
 def test_cache_memory():

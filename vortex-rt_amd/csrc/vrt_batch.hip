@@ -745,7 +745,7 @@ static int bd_create(vrt_g3* g, uint32_t max_seqs, uint32_t max_ctx, bool kv8, b
         B->q8 = static_cast<float*>(p);
         B->k8 = B->q8 + R * qw;
         B->v8 = B->k8 + R * hd;
-        if (int rc = bd_alloc(B, kv8_workspace_most(R, (hd + 31u) / 32u * 32u, R, H), &B->ws8)) return fail(rc);
+        if (int rc = bd_alloc(B, kv8_workspace_most(max_seqs, c.context_length, H, 1u, (hd + 31u) / 32u * 32u, evict), &B->ws8)) return fail(rc);
         if (evict) {
             if (int rc = bd_alloc(B, max_ctx * 4u, &p)) return fail(rc);
             B->kept = static_cast<uint32_t*>(p);

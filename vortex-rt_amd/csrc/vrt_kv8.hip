@@ -22,13 +22,12 @@ constexpr int kKvNoExp = -1000;   // no value scale yet
 // ---- layout ---------------------------------------------------------------------------------
 
 __device__ __forceinline__ uint64_t kv_block(const Kv8Dev& c, uint32_t seq, uint32_t head, uint32_t b) {
-    return (static_cast<uint64_t>(seq) * c.kvh + head) * c.nb + b % c.nb;
+    return (static_cast<uint64_t>(seq) * c.kvh + head) * c.nb + (b < c.nb ? b : b % c.nb);
 }
 __device__ __forceinline__ uint8_t* kv_codes(const Kv8Dev& c, uint64_t block) { return c.codes + block * 64u * c.hdp; }
-// Row (parity, K or V, slot) of the tail.
-__device__ __forceinline__ uint64_t kv_tail_row(const Kv8Dev& c, uint32_t seq, uint32_t head, uint32_t b, uint32_t z,
-                                                uint32_t slot) {
-    return (((static_cast<uint64_t>(seq) * c.kvh + head) * 2u + (b & 1u)) * 2u + z) * 32u + slot;
+// The tail buffer of block b's keys or values, of 32 rows.
+__device__ __forceinline__ uint64_t kv_tail_buf(const Kv8Dev& c, uint32_t seq, uint32_t head, uint32_t b, uint32_t z) {
+    return ((static_cast<uint64_t>(seq) * c.kvh + head) * 2u + (b & 1u)) * 2u + z;
 }
 // Byte of a value inside its block's 32 hdp bytes.
 __device__ __forceinline__ uint32_t kv_k_at(uint32_t t, uint32_t d) {
@@ -43,15 +42,28 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
     return v;
 }
 
+// x = hi + lo in f16 (x below 2^15 in magnitude; what is lost is below 2^-24)
+__device__ __forceinline__ void kv_split(float x, _Float16& hi, _Float16& lo) {
+    asm("" : "+v"(x));
+    hi = static_cast<_Float16>(x);
+    lo = static_cast<_Float16>(x - static_cast<float>(hi));
+}
+// The exponent e with m 2^e in [2^(to - 1), 2^to), at most 126 so that 2^-e is a number; 0 where m is 0 or not finite.
+__device__ __forceinline__ int kv_exp(float m, int to) {
+    return m > 0.0f && m < INFINITY ? min(to - __builtin_amdgcn_frexp_expf(m), 126) : 0;
+}
+
 // x / s to the nearest integer, ties to even, of the exact quotient: the remainder x - q s of the estimate is exact (q
 // has 8 bits, and it is below s), and says whether the estimate is one off.
 __device__ __forceinline__ float kv_round(float x, float s, float inv) {
 #pragma clang fp contract(off)
     float q = rintf(x * inv);
     const float r = __builtin_fmaf(-q, s, x), half = 0.5f * s;
-    const bool odd = static_cast<int>(q) & 1;
-    if (r > half || (r == half && odd)) q += 1.0f;
-    else if (r < -half || (r == -half && odd)) q -= 1.0f;
+    if (fabsf(r) >= half) {   // seldom
+        const bool odd = static_cast<int>(q) & 1;
+        if (r > half || (r == half && odd)) q += 1.0f;
+        else if (r < -half || (r == -half && odd)) q -= 1.0f;
+    }
     return fminf(fmaxf(q, -127.0f), 127.0f);
 }
 
@@ -62,8 +74,9 @@ __device__ __forceinline__ float kv_round(float x, float s, float inv) {
 struct KvTile {
     f4 v[8];
 };
+// (u / hd4 by a reciprocal: u below 2048, hd4 at most 64)
 __device__ __forceinline__ void kv_unit(uint32_t u, uint32_t hd4, uint32_t& t, uint32_t& d) {
-    t = u / hd4;
+    t = (u * ((1u << 20) / hd4 + 1u)) >> 20;
     d = (u - t * hd4) * 4u;
 }
 __device__ __forceinline__ uint32_t f_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
@@ -112,18 +125,56 @@ __device__ __forceinline__ void kv_close_block(const Kv8Dev& c, const KvTile& x,
     if (tid == 0u) reinterpret_cast<float*>(c.scales + block)[z] = s;
 }
 
-// Rows first .. last of block b (rows of x, which hold the call's positions from p0 on) into its tail: values and row maxima.
+// A tail row, held by a wave (lane l: dims 4 l ..): the fp32 row, and its pair of halves in operand order. The halves of a row
+// with a value that is not finite are zeros, so that what is masked adds nothing; its factor says so.
+__device__ __forceinline__ void kv_store_tail(const Kv8Dev& c, uint64_t buf, uint32_t z, uint32_t t, f4 v, bool rows) {
+    const uint32_t lane = threadIdx.x & 63u, d = 4u * lane;
+    const uint32_t m = wave_max_u32(max(max(f_bits(v[0]), f_bits(v[1])), max(f_bits(v[2]), f_bits(v[3]))));
+    const bool ok = m < 0x7f800000u;
+    const int ex = kv_exp(__uint_as_float(m), 7);
+    if (lane == 0u) c.factor[buf * 32u + t] = ok ? ldexpf(1.0f, -ex) : __uint_as_float(0x7fc00000u);
+    if (d >= c.hdp) return;
+    if (rows) *reinterpret_cast<f4*>(c.tail + (buf * 32u + t) * c.hdp + d) = v;
+    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+    h4 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        _Float16 a, b;
+        kv_split(ok ? ldexpf(v[e], ex) : 0.0f, a, b);
+        hi[e] = a;
+        lo[e] = b;
+    }
+    _Float16* dst = c.pairs + buf * 64u * c.hdp;
+    if (z == 0u) {
+        const uint32_t o = ((d >> 5) * 2u + (t >> 4)) * 512u + (((d >> 3) & 3u) * 16u + (t & 15u)) * 8u + (d & 7u);
+        *reinterpret_cast<h4*>(dst + o) = hi;
+        *reinterpret_cast<h4*>(dst + 32u * c.hdp + o) = lo;
+    } else {
+#pragma unroll
+        for (uint32_t e = 0; e < 4u; ++e) {
+            const uint32_t o = ((d + e) >> 4) * 512u + (((t >> 2) & 3u) * 16u + ((d + e) & 15u)) * 8u + (t & 3u) + (t >> 4) * 4u;
+            dst[o] = hi[e];
+            dst[32u * c.hdp + o] = lo[e];
+        }
+    }
+}
+
+// Positions first .. last of block b (rows of x, which hold the call's positions from p0 on) into its tail. A wave takes
+// every fourth, all of its rows loaded before the first is stored.
 __device__ __forceinline__ void kv_to_tail(const Kv8Dev& c, uint32_t seq, uint32_t head, uint32_t b, uint32_t z, const float* x,
                                            uint64_t stride, uint32_t p0, uint32_t first, uint32_t last) {
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    for (uint32_t p = first + wave; p <= last; p += kKvThreads / 64u) {
-        const uint64_t row = kv_tail_row(c, seq, head, b, z, p & 31u);
-        f4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (4u * lane < c.hd) v = *reinterpret_cast<const f4*>(x + static_cast<uint64_t>(p - p0) * stride + 4u * lane);
-        if (4u * lane < c.hdp) *reinterpret_cast<f4*>(c.tail + row * c.hdp + 4u * lane) = v;
-        const uint32_t m = wave_max_u32(max(max(f_bits(v[0]), f_bits(v[1])), max(f_bits(v[2]), f_bits(v[3]))));
-        if (lane == 0u) c.tmax[row] = __uint_as_float(m);
+    f4 v[8];
+#pragma unroll
+    for (uint32_t k = 0; k < 8u; ++k) {
+        const uint32_t p = first + wave + 4u * k;
+        v[k] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (p <= last && 4u * lane < c.hd) v[k] = *reinterpret_cast<const f4*>(x + static_cast<uint64_t>(p - p0) * stride + 4u * lane);
     }
+    const uint64_t buf = kv_tail_buf(c, seq, head, b, z);
+#pragma unroll
+    for (uint32_t k = 0; k < 8u; ++k)
+        if (first + wave + 4u * k <= last) kv_store_tail(c, buf, z, (first + wave + 4u * k) & 31u, v[k], true);
 }
 
 struct Kv8AppendArgs {
@@ -134,8 +185,8 @@ struct Kv8AppendArgs {
 };
 
 // One workgroup per (block the call touches, head and K or V, sequence). A full block's codes; the rows of the last two
-// blocks also go to the tail. The first block's earlier rows come from the tail, which a later block of the same
-// parity would overwrite: so the first block's workgroup writes all of the tail, after it has read it.
+// blocks also go to the tail. The first block's earlier rows come from the tail, which a later block of the same parity
+// overwrites: the first block's workgroup writes that one's rows too, after it has read its own.
 __global__ void __launch_bounds__(kKvThreads) k_kv8_append(const Kv8AppendArgs A) {
     __shared__ __align__(16) uint8_t img[32 * 256];
     __shared__ uint32_t red[4];
@@ -150,6 +201,7 @@ __global__ void __launch_bounds__(kKvThreads) k_kv8_append(const Kv8AppendArgs A
     if (closed) {
         KvTile T;
         const uint32_t hd4 = c.hd >> 2, units = 32u * hd4;
+        const float* old = c.tail + kv_tail_buf(c, S.seq, head, b, z) * 32u * c.hdp;
 #pragma unroll
         for (uint32_t k = 0; k < 8u; ++k) {
             const uint32_t u = tid + kKvThreads * k;
@@ -158,15 +210,16 @@ __global__ void __launch_bounds__(kKvThreads) k_kv8_append(const Kv8AppendArgs A
             uint32_t t, d;
             kv_unit(u, hd4, t, d);
             const uint32_t p = 32u * b + t;
-            const float* src = p < S.pos ? c.tail + kv_tail_row(c, S.seq, head, b, z, t) * c.hdp + d
-                                         : x + static_cast<uint64_t>(p - S.pos) * A.stride + d;
-            T.v[k] = *reinterpret_cast<const f4*>(src);
+            T.v[k] = *reinterpret_cast<const f4*>(p < S.pos ? old + t * c.hdp + d : x + static_cast<uint64_t>(p - S.pos) * A.stride + d);
         }
         kv_close_block(c, T, kv_block(c, S.seq, head, b), z, img, red);   // (its barriers come after every read of the tail)
     }
-    if (b != b0) return;
-    for (uint32_t t = bl > b0 ? bl - 1u : bl; t <= bl; ++t)
-        kv_to_tail(c, S.seq, head, t, z, x, A.stride, S.pos, max(S.pos, 32u * t), min(end, 32u * t + 32u) - 1u);
+    const bool shared = (S.pos & 31u) != 0u;   // the first block reads its tail
+    for (uint32_t t = bl > b0 ? bl - 1u : bl; t <= bl; ++t) {
+        const bool firsts = t == b0 || (shared && ((t ^ b0) & 1u) == 0u);
+        if (firsts ? b == b0 : b == t)
+            kv_to_tail(c, S.seq, head, t, z, x, A.stride, S.pos, max(S.pos, 32u * t), min(end, 32u * t + 32u) - 1u);
+    }
 }
 
 // ---- read -----------------------------------------------------------------------------------
@@ -182,26 +235,47 @@ __device__ __forceinline__ float kv_value(const Kv8Dev& c, uint32_t seq, uint32_
                                           uint32_t len) {
 #pragma clang fp contract(off)
     const uint32_t b = p >> 5, t = p & 31u;
-    if ((b + 1u) * 32u > len) return c.tail[kv_tail_row(c, seq, head, b, z, t) * c.hdp + d];
+    if ((b + 1u) * 32u > len) return c.tail[(kv_tail_buf(c, seq, head, b, z) * 32u + t) * c.hdp + d];
     const uint64_t blk = kv_block(c, seq, head, b);
     const uint8_t u = kv_codes(c, blk)[z * 32u * c.hdp + (z ? kv_v_at(t, d) : kv_k_at(t, d))];
     const float s = reinterpret_cast<const float*>(c.scales + blk)[z];
     return s * static_cast<float>(static_cast<int>(u) - 128);
 }
 
+// One workgroup per (block, head and K or V, sequence): the block's codes in 16-byte units into LDS, rows out of it.
 __global__ void __launch_bounds__(kKvThreads) k_kv8_read(const Kv8ReadArgs A) {
+#pragma clang fp contract(off)
+    __shared__ __align__(16) uint8_t img[32 * 256];
     const Kv8Dev& c = A.c;
     const Kv8Seq& S = A.s[blockIdx.z];
-    const uint32_t head = blockIdx.y >> 1, z = blockIdx.y & 1u;
+    const uint32_t head = blockIdx.y >> 1, z = blockIdx.y & 1u, tid = threadIdx.x;
     const uint32_t b = (S.pos >> 5) + blockIdx.x, hd4 = c.hd >> 2;
-    for (uint32_t u = threadIdx.x; u < 32u * hd4; u += kKvThreads) {
+    if (S.n == 0u || b > (S.pos + S.n - 1u) >> 5) return;
+    const bool closed = (b + 1u) * 32u <= S.prefix;
+    float s = 0.0f;
+    if (closed) {
+        const uint64_t blk = kv_block(c, S.seq, head, b);
+        const uint4* src = reinterpret_cast<const uint4*>(kv_codes(c, blk) + z * 32u * c.hdp);
+        s = reinterpret_cast<const float*>(c.scales + blk)[z];
+        for (uint32_t i = tid; i < 2u * c.hdp; i += kKvThreads) reinterpret_cast<uint4*>(img)[i] = src[i];
+        __syncthreads();
+    }
+    const float* old = c.tail + kv_tail_buf(c, S.seq, head, b, z) * 32u * c.hdp;
+    for (uint32_t u = tid; u < 32u * hd4; u += kKvThreads) {
         uint32_t t, d;
         kv_unit(u, hd4, t, d);
         const uint32_t p = 32u * b + t;
         if (p < S.pos || p - S.pos >= S.n) continue;
         f4 v;
+        if (closed) {
+            uint32_t w;
+            if (z == 0u) w = *reinterpret_cast<const uint32_t*>(img + kv_k_at(t, d));
+            else w = img[kv_v_at(t, d)] | img[kv_v_at(t, d + 1u)] << 8 | img[kv_v_at(t, d + 2u)] << 16 | img[kv_v_at(t, d + 3u)] << 24;
 #pragma unroll
-        for (uint32_t e = 0; e < 4u; ++e) v[e] = kv_value(c, S.seq, head, z, p, d + e, S.prefix);
+            for (uint32_t e = 0; e < 4u; ++e) v[e] = s * static_cast<float>(static_cast<int>((w >> (8u * e)) & 255u) - 128);
+        } else {
+            v = *reinterpret_cast<const f4*>(old + t * c.hdp + d);
+        }
         *reinterpret_cast<f4*>(A.x[z] + (static_cast<uint64_t>(S.row0) + (p - S.pos)) * A.stride + head * c.hd + d) = v;
     }
 }
@@ -235,17 +309,6 @@ __device__ __forceinline__ h8 kv_cvt8(uint32_t w0, uint32_t w1) {
     return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// x = hi + lo in f16 (x below 2^15 in magnitude; what is lost is below 2^-24)
-__device__ __forceinline__ void kv_split(float x, _Float16& hi, _Float16& lo) {
-    asm("" : "+v"(x));
-    hi = static_cast<_Float16>(x);
-    lo = static_cast<_Float16>(x - static_cast<float>(hi));
-}
-// The exponent e with m 2^e in [2^(to - 1), 2^to), at most 126 so that 2^-e is a number; 0 where m is 0 or not finite.
-__device__ __forceinline__ int kv_exp(float m, int to) {
-    return m > 0.0f && m < INFINITY ? min(to - __builtin_amdgcn_frexp_expf(m), 126) : 0;
-}
-
 // tanh(x): below 1/4 its series (the next term is 9e-9 of it), above by e^(-2|x|), at 1 ulp each of exponential and
 // reciprocal.
 __device__ __forceinline__ float kv_tanh(float x) {
@@ -256,119 +319,269 @@ __device__ __forceinline__ float kv_tanh(float x) {
     return a < 0.25f ? small : copysignf(big, x);
 }
 
-// A row tile's queries as the B operand of the transposed scores: lane l holds row r0 + l % 16 (query (r0 + l % 16) / G, head
-// kvh G + (r0 + l % 16) % G), dims 32 s + 8 (l / 16) + e, scaled by a power of two to below 2^14 and split.
-template <int NT>
-struct KvQuery {
-    h8 hi[NT], lo[NT];
-    float back;    // the row's power of two, inverted
-    uint32_t p;    // its position
-};
-template <int NT>
-__device__ __forceinline__ void kv_load_q(const Kv8AttnArgs& A, const Kv8Seq& S, uint32_t kvh, uint32_t r0, KvQuery<NT>& Q) {
-    const uint32_t lane = threadIdx.x & 63u, R = S.n * A.G, hd = A.c.hd;
-    const uint32_t r = min(r0 + (lane & 15u), R - 1u), qi = r / A.G, h = kvh * A.G + (r - qi * A.G);
-    const float* src = A.q + (static_cast<uint64_t>(S.row0) + qi) * A.q_stride + h * hd;
-    f4 x[NT][2];
-    float m = 0.0f;
-#pragma unroll
-    for (int s = 0; s < NT; ++s)
-#pragma unroll
-        for (uint32_t j = 0; j < 2u; ++j) {
-            const uint32_t d = 32u * s + 8u * (lane >> 4) + 4u * j;
-            x[s][j] = d < hd ? *reinterpret_cast<const f4*>(src + d) : f4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(x[s][j][e]));
-        }
-    m = fmaxf(m, __shfl_xor(m, 16));
-    m = fmaxf(m, __shfl_xor(m, 32));
-    const int ex = kv_exp(m, 14);
-    Q.back = ldexpf(1.0f, -ex);
-    Q.p = S.pos + qi;
-#pragma unroll
-    for (int s = 0; s < NT; ++s)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            _Float16 a, b;
-            kv_split(ldexpf(x[s][j >> 2][j & 3], ex), a, b);
-            Q.hi[s][j] = a;
-            Q.lo[s][j] = b;
-        }
-}
-
 #define KV_MFMA(a, b, c) __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0)
 
-// Block b's scores, in log2 units and masked: lane l holds row l % 16's of tokens 4 (l / 16) + e (e < 4) and 16 + 4 (l / 16) + e - 4.
-// Of the sequence's open block the keys come from the tail, as f16 pairs; tmax names their largest and those not finite.
-template <int NT, bool CAP>
-__device__ __forceinline__ void kv_scores(const Kv8AttnArgs& A, const Kv8Seq& S, uint32_t kvh, uint32_t b, const KvQuery<NT>& Q,
-                                          bool masked, float (&s)[8]) {
-    const Kv8Dev& c = A.c;
-    const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, m16 = lane & 15u, len = S.pos + S.n;
-    f4 acc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
-    float ks;
-    if ((b + 1u) * 32u <= len) {
-        const uint64_t blk = kv_block(c, S.seq, kvh, b);
-        const uint4* src = reinterpret_cast<const uint4*>(kv_codes(c, blk)) + lane;
-        ks = c.scales[blk].x;
+__device__ __forceinline__ float max_xor16(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float max_xor32(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// What a wave holds of RT tiles of 16 query rows (lane l: row l % 16 of each). The queries are the B operand of the transposed
+// scores (lane l: dims 32 s + 8 (l / 16) + e), scaled by a power of two to below 2^14 and split into halves. The outputs are
+// transposed too (dims 16 t + 4 (l / 16) + e), in units of 2^(eR - 9).
+constexpr float kKvGrow = 6.0f;   // weights may pass 1 by 2^6 before the reference maximum follows
+template <int NT, int RT>
+struct KvWave {
+    h8 qh[RT][NT], ql[RT][NT];
+    f4 acc[RT][2 * NT];
+    float f[RT];      // a score's factor but for its key's scale
+    uint32_t p[RT];   // the rows' positions
+    float m[RT], l[RT];
+    int eR;           // 2^eR is above every value scale so far
+};
+
+template <int NT, int RT, bool CAP>
+__device__ __forceinline__ void kv_start(const Kv8AttnArgs& A, const Kv8Seq& S, uint32_t kvh, uint32_t r0, KvWave<NT, RT>& W) {
+    const uint32_t lane = threadIdx.x & 63u, R = S.n * A.G, hd = A.c.hd;
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const uint4 w = src[64 * t];
-            const h8 a0 = kv_cvt8(w.x, w.y), a1 = kv_cvt8(w.z, w.w);
-            acc[0] = KV_MFMA(a0, Q.hi[t], acc[0]);
-            acc[1] = KV_MFMA(a1, Q.hi[t], acc[1]);
-            acc[0] = KV_MFMA(a0, Q.lo[t], acc[0]);
-            acc[1] = KV_MFMA(a1, Q.lo[t], acc[1]);
-        }
-    } else {
-        const uint64_t row0 = kv_tail_row(c, S.seq, kvh, b, 0u, 0u);
-        const uint32_t live = len - 32u * b;   // tokens of the block
-        float m = (lane & 31u) < live ? c.tmax[row0 + (lane & 31u)] : 0.0f;
-        m = wave_max(m < INFINITY ? m : 0.0f);
-        const int ex = kv_exp(m, 7);
-        ks = ldexpf(1.0f, -ex);
+    for (int k = 0; k < RT; ++k) {
+        const uint32_t r = min(r0 + 16u * k + (lane & 15u), R - 1u), qi = r / A.G, h = kvh * A.G + (r - qi * A.G);
+        const float* src = A.q + (static_cast<uint64_t>(S.row0) + qi) * A.q_stride + h * hd;
+        f4 x[NT][2];
+        float m = 0.0f;
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+        for (int s = 0; s < NT; ++s)
 #pragma unroll
-            for (uint32_t half = 0; half < 2u; ++half) {
-                const uint32_t tok = 16u * half + m16;
-                h8 hi, lo;
-                f4 x[2];
-#pragma unroll
-                for (uint32_t j = 0; j < 2u; ++j)
-                    x[j] = *reinterpret_cast<const f4*>(c.tail + (row0 + min(tok, live - 1u)) * c.hdp + 32u * t + 8u * g + 4u * j);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    _Float16 h, l;
-                    kv_split(ldexpf(x[j >> 2][j & 3], ex), h, l);
-                    hi[j] = h;
-                    lo[j] = l;
-                }
-                acc[half] = KV_MFMA(hi, Q.hi[t], acc[half]);
-                acc[half] = KV_MFMA(hi, Q.lo[t], acc[half]);
-                acc[half] = KV_MFMA(lo, Q.hi[t], acc[half]);
+            for (uint32_t j = 0; j < 2u; ++j) {
+                const uint32_t d = 32u * s + 8u * (lane >> 4) + 4u * j;
+                x[s][j] = d < hd ? *reinterpret_cast<const f4*>(src + d) : f4{0.0f, 0.0f, 0.0f, 0.0f};
             }
-    }
-    const float f = Q.back * (ks * A.scale);
 #pragma unroll
-    for (uint32_t e = 0; e < 8u; ++e) {
-        float x = acc[e >> 2][e & 3u];
-        if constexpr (CAP) x = A.cap * kv_tanh(x * f * (1.0f / A.cap)) * 1.4426950409f;
-        else x = x * (f * 1.4426950409f);
-        if (masked) {
-            const uint32_t j = 32u * b + 4u * g + (e & 3u) + 16u * (e >> 2);
-            const bool see = j < len && (j < S.prefix || (j <= Q.p && (!A.window || Q.p - j < A.window)));
-            x = see ? x : -INFINITY;
+        for (int s = 0; s < NT; ++s)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(x[s][j >> 2][j & 3]));
+        m = max_xor32(max_xor16(m));
+        const int ex = kv_exp(m, 14);
+        const float sign = A.scale < 0.0f ? -1.0f : 1.0f;   // factors are not negative: the largest score is the largest product
+        W.f[k] = ldexpf(1.0f, -ex) * (fabsf(A.scale) * (CAP ? 1.0f : 1.4426950409f));
+        W.p[k] = S.pos + qi;
+        W.m[k] = -INFINITY;
+        W.l[k] = 0.0f;
+#pragma unroll
+        for (int s = 0; s < NT; ++s)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                _Float16 a, b;
+                kv_split(ldexpf(x[s][j >> 2][j & 3] * sign, ex), a, b);
+                W.qh[k][s][j] = a;
+                W.ql[k][s][j] = b;
+            }
+#pragma unroll
+        for (int t = 0; t < 2 * NT; ++t) W.acc[k][t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    W.eR = kKvNoExp;
+}
+
+// A full block's codes in registers: lane l's 16 bytes of each 32 dims.
+template <int NT>
+struct KvRaw {
+    uint4 w[NT];
+};
+template <int NT>
+__device__ __forceinline__ void kv_load(const Kv8Dev& c, uint64_t blk, uint32_t z, KvRaw<NT>& r) {
+    const uint4* src = reinterpret_cast<const uint4*>(kv_codes(c, blk) + z * 32u * c.hdp) + (threadIdx.x & 63u);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) r.w[t] = src[64 * t];
+}
+
+// Products of 32 tokens' keys with the queries: s[k][half], lane l: row l % 16, tokens 16 half + 4 (l / 16) + e.
+template <int NT, int RT>
+__device__ __forceinline__ void kv_scores(const KvRaw<NT>& K, const KvWave<NT, RT>& W, f4 (&s)[RT][2]) {
+#pragma unroll
+    for (int k = 0; k < RT; ++k) s[k][0] = s[k][1] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const h8 a0 = kv_cvt8(K.w[t].x, K.w[t].y), a1 = kv_cvt8(K.w[t].z, K.w[t].w);
+#pragma unroll
+        for (int k = 0; k < RT; ++k) {
+            s[k][0] = KV_MFMA(a0, W.qh[k][t], s[k][0]);
+            s[k][1] = KV_MFMA(a1, W.qh[k][t], s[k][1]);
         }
-        s[e] = x;
+#pragma unroll
+        for (int k = 0; k < RT; ++k) {
+            s[k][0] = KV_MFMA(a0, W.ql[k][t], s[k][0]);
+            s[k][1] = KV_MFMA(a1, W.ql[k][t], s[k][1]);
+        }
+    }
+}
+// The same of the open block, from the tail's pairs.
+template <int NT, int RT>
+__device__ __forceinline__ void kv_scores_open(const Kv8Dev& c, uint64_t buf, const KvWave<NT, RT>& W, f4 (&s)[RT][2]) {
+    const h8* hi = reinterpret_cast<const h8*>(c.pairs + buf * 64u * c.hdp) + (threadIdx.x & 63u);
+    const h8* lo = hi + 4u * c.hdp;
+#pragma unroll
+    for (int k = 0; k < RT; ++k) s[k][0] = s[k][1] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const h8 a = hi[64 * (2 * t + half)], b = lo[64 * (2 * t + half)];
+#pragma unroll
+            for (int k = 0; k < RT; ++k) {
+                s[k][half] = KV_MFMA(a, W.qh[k][t], s[k][half]);
+                s[k][half] = KV_MFMA(a, W.ql[k][t], s[k][half]);
+                s[k][half] = KV_MFMA(b, W.qh[k][t], s[k][half]);
+            }
+        }
+}
+
+// Tokens of a lane's eight scores.
+__device__ __forceinline__ uint32_t kv_token(uint32_t e) { return 4u * ((threadIdx.x & 63u) >> 4) + (e & 3u) + 16u * (e >> 2); }
+
+// One block's scores to weights: x in log2 units, running reference maximum and sum, the weights times the values'
+// scale as pairs of halves. ks / vs: the block's scales, or (OPEN) those of the lane's tokens. dump: where the row's scores go.
+template <int NT, int RT, bool CAP, bool OPEN>
+__device__ __forceinline__ void kv_soft(const Kv8AttnArgs& A, const Kv8Seq& S, uint32_t b, bool masked, const f4 (&s)[RT][2],
+                                        const float* ks, const float* vs, KvWave<NT, RT>& W, h8 (&ph)[RT], h8 (&pl)[RT], float* dump) {
+    float x[RT][8], top[RT];
+    uint32_t see[RT];   // bit e
+#pragma unroll
+    for (int k = 0; k < RT; ++k) {
+        see[k] = 0xffu;
+        if (masked) {
+            see[k] = 0u;
+            const uint32_t len = S.pos + S.n;
+#pragma unroll
+            for (uint32_t e = 0; e < 8u; ++e) {
+                const uint32_t j = 32u * b + kv_token(e);
+                const bool y = j < len && (j < S.prefix || (j <= W.p[k] && (!A.window || W.p[k] - j < A.window)));
+                see[k] |= static_cast<uint32_t>(y) << e;
+            }
+        }
+        top[k] = -INFINITY;
+#pragma unroll
+        for (uint32_t e = 0; e < 8u; ++e) {
+            x[k][e] = s[k][e >> 2][e & 3u] * (W.f[k] * (OPEN ? ks[e] : ks[0]));
+            if constexpr (CAP) x[k][e] = A.cap * 1.4426950409f * kv_tanh(x[k][e] * (1.0f / A.cap));
+            if (masked) x[k][e] = (see[k] >> e) & 1u ? x[k][e] : -INFINITY;
+            top[k] = fmaxf(top[k], x[k][e]);
+        }
+        top[k] = max_xor32(max_xor16(top[k]));
+    }
+    float v = OPEN ? 0.0f : vs[0];
+    if constexpr (OPEN) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v = fmaxf(v, vs[e]);
+        v = max_xor32(max_xor16(v));
+    }
+    const int ev = v > 0.0f && v < INFINITY ? __builtin_amdgcn_frexp_expf(v) : kKvNoExp;
+    bool grow = ev > W.eR;
+#pragma unroll
+    for (int k = 0; k < RT; ++k) grow |= top[k] > W.m[k] + kKvGrow;
+    if (__any(grow)) {
+        const int eR = max(W.eR, ev);
+#pragma unroll
+        for (int k = 0; k < RT; ++k) {
+            const float m = top[k] > W.m[k] + kKvGrow ? top[k] : W.m[k];
+            const float beta = m == W.m[k] ? 1.0f : __builtin_amdgcn_exp2f(W.m[k] - m);
+            const float alpha = ldexpf(beta, W.eR - eR);
+            W.m[k] = m;
+            W.l[k] *= beta;
+#pragma unroll
+            for (int t = 0; t < 2 * NT; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) W.acc[k][t][e] *= alpha;
+        }
+        W.eR = eR;
+    }
+    const int up = W.eR == kKvNoExp ? 0 : 9 - W.eR;
+#pragma unroll
+    for (int k = 0; k < RT; ++k) {
+        const float ref = W.m[k] == -INFINITY ? 0.0f : W.m[k];
+        float p[8];
+#pragma unroll
+        for (uint32_t e = 0; e < 8u; ++e) {
+            p[e] = __builtin_amdgcn_exp2f(x[k][e] - ref);
+            W.l[k] += p[e];
+            p[e] *= ldexpf(OPEN ? vs[e] : vs[0], up);
+            if (masked) p[e] = (see[k] >> e) & 1u ? p[e] : 0.0f;   // (0 times a scale that is NaN)
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            _Float16 a, d;
+            kv_split(p[e], a, d);
+            ph[k][e] = a;
+            pl[k][e] = d;
+        }
+    }
+    if (dump) {
+        *reinterpret_cast<f4*>(dump) = f4{x[0][0], x[0][1], x[0][2], x[0][3]};
+        *reinterpret_cast<f4*>(dump + 16) = f4{x[0][4], x[0][5], x[0][6], x[0][7]};
     }
 }
 
-// Whether some row of a tile does not see all of block b.
+template <int NT, int RT>
+__device__ __forceinline__ void kv_values(const KvRaw<NT>& V, const h8 (&ph)[RT], const h8 (&pl)[RT], KvWave<NT, RT>& W) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const h8 a0 = kv_cvt8(V.w[t].x, V.w[t].y), a1 = kv_cvt8(V.w[t].z, V.w[t].w);
+#pragma unroll
+        for (int k = 0; k < RT; ++k) {
+            W.acc[k][2 * t] = KV_MFMA(a0, ph[k], W.acc[k][2 * t]);
+            W.acc[k][2 * t + 1] = KV_MFMA(a1, ph[k], W.acc[k][2 * t + 1]);
+        }
+#pragma unroll
+        for (int k = 0; k < RT; ++k) {
+            W.acc[k][2 * t] = KV_MFMA(a0, pl[k], W.acc[k][2 * t]);
+            W.acc[k][2 * t + 1] = KV_MFMA(a1, pl[k], W.acc[k][2 * t + 1]);
+        }
+    }
+}
+
+// The open block of a sequence (its last): live rows of the tail; what lies past them is whatever the memory held.
+template <int NT, int RT, bool CAP>
+__device__ __forceinline__ void kv_open(const Kv8AttnArgs& A, const Kv8Seq& S, uint32_t kvh, uint32_t b, KvWave<NT, RT>& W, float* dump) {
+    const Kv8Dev& c = A.c;
+    const uint32_t lane = threadIdx.x & 63u, live = S.pos + S.n - 32u * b;
+    const uint64_t kb = kv_tail_buf(c, S.seq, kvh, b, 0u), vb = kb + 1u;
+    float ks[8], vs[8];
+    uint32_t keep[4];   // of the values' operand: halves 2 i and 2 i + 1
+#pragma unroll
+    for (uint32_t e = 0; e < 8u; ++e) {
+        const bool y = kv_token(e) < live;
+        ks[e] = y ? c.factor[kb * 32u + kv_token(e)] : 0.0f;
+        vs[e] = y ? c.factor[vb * 32u + kv_token(e)] : 0.0f;
+        keep[e >> 1] = (e & 1u ? keep[e >> 1] : 0u) | (y ? 0xffffu << (16u * (e & 1u)) : 0u);
+    }
+    f4 s[RT][2];
+    h8 ph[RT], pl[RT];
+    kv_scores_open<NT, RT>(c, kb, W, s);
+    kv_soft<NT, RT, CAP, true>(A, S, b, true, s, ks, vs, W, ph, pl, dump);
+    const uint4* hi = reinterpret_cast<const uint4*>(c.pairs + vb * 64u * c.hdp) + lane;
+    const uint4* lo = hi + 4u * c.hdp;
+#pragma unroll
+    for (int t = 0; t < 2 * NT; ++t) {
+        uint4 x = hi[64 * t], y = lo[64 * t];
+        x.x &= keep[0], x.y &= keep[1], x.z &= keep[2], x.w &= keep[3];
+        y.x &= keep[0], y.y &= keep[1], y.z &= keep[2], y.w &= keep[3];
+        const h8 a = __builtin_bit_cast(h8, x), d = __builtin_bit_cast(h8, y);
+#pragma unroll
+        for (int k = 0; k < RT; ++k) {
+            W.acc[k][t] = KV_MFMA(a, ph[k], W.acc[k][t]);
+            W.acc[k][t] = KV_MFMA(a, pl[k], W.acc[k][t]);
+            W.acc[k][t] = KV_MFMA(d, ph[k], W.acc[k][t]);
+        }
+    }
+}
+
+// Whether some row at positions pmin .. pmax does not see all of the full block b.
 __device__ __forceinline__ bool kv_masked(const Kv8AttnArgs& A, const Kv8Seq& S, uint32_t b, uint32_t pmin, uint32_t pmax) {
-    const uint32_t last = 32u * b + 31u, len = S.pos + S.n;
-    if (last < S.prefix && last < len) return false;
-    return !(last <= pmin && (!A.window || pmax - 32u * b < A.window));
+    const uint32_t last = 32u * b + 31u;
+    return last >= S.prefix && (last > pmin || (A.window && pmax - 32u * b >= A.window));
 }
 
 // Four outputs of (row, head), and what is left to say of it.
@@ -396,230 +609,296 @@ __device__ __forceinline__ void kv_row_done(const Kv8AttnArgs& A, uint32_t row, 
     if (A.o.nonfinite && (!(L > 0.0f) || !__builtin_isfinite(L))) atomicMin(A.o.nonfinite, A.o.code);
 }
 
-// One workgroup per (split of a row tile's blocks, head, sequence); wave w takes the split's blocks w, w + 4, ...: scores on
-// the matrix cores with the tokens as rows, so that each lane holds eight weights of one query row in the order in
-// which the values are kept; running maximum and sum per row; weights times the block's value scale, as f16 pairs, times
-// the values' codes into the transposed output (rows: dims). The waves meet in LDS.
+// The virtual blocks i0, i0 + step, ... below i1 of a wave's rows (span sp). The keys of the next block are loaded while
+// this one's weights are computed, its values while the next scores are.
+template <int NT, int RT, bool CAP>
+__device__ __forceinline__ void kv_run(const Kv8AttnArgs& A, const Kv8Seq& S, uint32_t kvh, const KvSpan& sp, uint32_t pmin, uint32_t pmax,
+                                       uint32_t i0, uint32_t i1, uint32_t step, KvWave<NT, RT>& W, float* dump) {
+    const Kv8Dev& c = A.c;
+    auto block = [&](uint32_t i) { return i < sp.n_pre ? i : sp.lo + (i - sp.n_pre); };
+    const uint32_t last = block(sp.n - 1u);
+    const bool open = (last + 1u) * 32u > S.pos + S.n;   // the last virtual block
+    const uint32_t e1 = open ? min(i1, sp.n - 1u) : i1;
+    uint32_t i = i0;
+    if (i < e1) {
+        KvRaw<NT> K, V;
+        uint64_t blk = kv_block(c, S.seq, kvh, block(i));
+        kv_load<NT>(c, blk, 0u, K);
+        kv_load<NT>(c, blk, 1u, V);
+        float2 sc = c.scales[blk];
+        for (; i < e1; i += step) {
+            const uint32_t b = block(i);
+            f4 s[RT][2];
+            kv_scores<NT, RT>(K, W, s);
+            const bool more = i + step < e1;
+            const float2 cur = sc;
+            if (more) {
+                blk = kv_block(c, S.seq, kvh, block(i + step));
+                kv_load<NT>(c, blk, 0u, K);
+                sc = c.scales[blk];
+            }
+            h8 ph[RT], pl[RT];
+            kv_soft<NT, RT, CAP, false>(A, S, b, kv_masked(A, S, b, pmin, pmax), s, &cur.x, &cur.y, W, ph, pl,
+                                        dump ? dump + 32u * (i - i0) : nullptr);
+            kv_values<NT, RT>(V, ph, pl, W);
+            if (more) kv_load<NT>(c, blk, 1u, V);
+        }
+    }
+    if (open && i == sp.n - 1u && i < i1) kv_open<NT, RT, CAP>(A, S, kvh, last, W, dump ? dump + 32u * (i - i0) : nullptr);
+}
+
+// Single tokens, and a few: one workgroup per (split of a 16-row unit's blocks, head, sequence), its waves taking every fourth
+// block and meeting in LDS, eight rows at a time.
 template <int NT, bool CAP>
-__global__ void __launch_bounds__(kKvThreads) k_kv8_attn(const Kv8AttnArgs A) {
-    constexpr uint32_t kRow = 32u * NT + 4u;
-    __shared__ __align__(16) float s_acc[2][16 * kRow];
+__global__ void __launch_bounds__(kKvThreads, 2) k_kv8_attn(const Kv8AttnArgs A) {
+    constexpr uint32_t HDP = 32u * NT, C4 = HDP / 4u;
+    __shared__ __align__(16) f4 s_acc[4][8 * C4];
     __shared__ float s_m[4][16], s_l[4][16];
     const Kv8Seq& S = A.s[blockIdx.z];
-    const uint32_t kvh = blockIdx.y, tile = blockIdx.x / A.splits, split = blockIdx.x - tile * A.splits;
-    const uint32_t R = S.n * A.G, r0 = 16u * tile, len = S.pos + S.n;
+    const uint32_t kvh = blockIdx.y, unit = blockIdx.x / A.splits, split = blockIdx.x - unit * A.splits;
+    const uint32_t R = S.n * A.G, r0 = 16u * unit;
     if (r0 >= R || split >= S.splits) return;
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, m16 = lane & 15u;
     const uint32_t pmin = S.pos + r0 / A.G, pmax = S.pos + min(r0 + 15u, R - 1u) / A.G;
     const KvSpan sp = kv_span(A, S, pmin, pmax);
-    const uint32_t i0 = split * A.per, i1 = min(sp.n, i0 + A.per);
+    const uint32_t i0 = split * A.per, i1 = min(sp.n, i0 + A.per), rows = min(16u, R - r0);
     if (i0 >= i1) return;
-    const Kv8Dev& c = A.c;
-    KvQuery<NT> Q;
-    kv_load_q<NT>(A, S, kvh, r0, Q);
-    float m = -INFINITY, l = 0.0f;
-    int eR = kKvNoExp;   // acc holds sum p v 2^(15 - eR), 2^eR above every value scale so far
-    f4 acc[2 * NT];
-#pragma unroll
-    for (int t = 0; t < 2 * NT; ++t) acc[t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint32_t i = i0 + wave; i < i1; i += 4u) {
-        const uint32_t b = i < sp.n_pre ? i : sp.lo + (i - sp.n_pre);
-        const bool open = (b + 1u) * 32u > len;
-        float s[8];
-        kv_scores<NT, CAP>(A, S, kvh, b, Q, open || kv_masked(A, S, b, pmin, pmax), s);
-        // the block's value scale; of the open block: a power of two, and its tokens with a key or value that is not finite
-        const uint64_t row0 = kv_tail_row(c, S.seq, kvh, b, 1u, 0u);
-        const uint32_t live = min(32u, len - 32u * b);
-        float vs;
-        int tex = 0;
-        uint32_t bad = 0u;
-        if (!open) {
-            vs = c.scales[kv_block(c, S.seq, kvh, b)].y;
-        } else {
-            const float tv = (lane & 31u) < live ? c.tmax[row0 + (lane & 31u)] : 0.0f;
-            const float tk = (lane & 31u) < live ? c.tmax[kv_tail_row(c, S.seq, kvh, b, 0u, lane & 31u)] : 0.0f;
-            bad = static_cast<uint32_t>(__ballot(!(tv < INFINITY) || !(tk < INFINITY)));
-            tex = kv_exp(wave_max(tv < INFINITY ? tv : 0.0f), 7);
-            vs = ldexpf(1.0f, -tex);
-        }
-        float mx = m;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) mx = fmaxf(mx, s[e]);
-        mx = fmaxf(mx, __shfl_xor(mx, 16));
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const float ref = mx == -INFINITY ? 0.0f : mx;
-        const float beta = __builtin_amdgcn_exp2f(m - ref);
-        m = mx;
-        const int ev = vs > 0.0f && vs < INFINITY ? __builtin_amdgcn_frexp_expf(vs) : kKvNoExp;
-        const float alpha = ev > eR ? (eR == kKvNoExp ? 0.0f : ldexpf(beta, eR - ev)) : beta;
-        const bool first = eR == kKvNoExp;
-        eR = max(eR, ev);
-        const float f = eR == kKvNoExp ? vs : ldexpf(vs, 15 - eR);
-        h8 ph, pl;
-        l *= beta;
-#pragma unroll
-        for (uint32_t e = 0; e < 8u; ++e) {
-            const uint32_t tok = 4u * g + (e & 3u) + 16u * (e >> 2);
-            const bool see = s[e] != -INFINITY;
-            float p = __builtin_amdgcn_exp2f(s[e] - ref);
-            if (see && ((bad >> tok) & 1u)) p = __uint_as_float(0x7fc00000u);
-            l += p;
-            _Float16 a, d;
-            kv_split(see ? p * f : 0.0f, a, d);
-            ph[e] = a;
-            pl[e] = d;
-        }
-        if (!first)
-#pragma unroll
-            for (int t = 0; t < 2 * NT; ++t)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[t][e] *= alpha;
-        if (!open) {
-            const uint4* src = reinterpret_cast<const uint4*>(kv_codes(c, kv_block(c, S.seq, kvh, b)) + 32u * c.hdp) + lane;
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const uint4 w = src[64 * t];
-                const h8 a0 = kv_cvt8(w.x, w.y), a1 = kv_cvt8(w.z, w.w);
-                acc[2 * t] = KV_MFMA(a0, ph, acc[2 * t]);
-                acc[2 * t + 1] = KV_MFMA(a1, ph, acc[2 * t + 1]);
-                acc[2 * t] = KV_MFMA(a0, pl, acc[2 * t]);
-                acc[2 * t + 1] = KV_MFMA(a1, pl, acc[2 * t + 1]);
-            }
-        } else {
-#pragma unroll
-            for (int t = 0; t < 2 * NT; ++t) {
-                h8 hi, lo;
-#pragma unroll
-                for (uint32_t e = 0; e < 8u; ++e) {
-                    const uint32_t tok = 4u * g + (e & 3u) + 16u * (e >> 2);
-                    float x = c.tail[(row0 + min(tok, live - 1u)) * c.hdp + 16u * t + m16];
-                    if (tok >= live || ((bad >> tok) & 1u)) x = 0.0f;   // 0 x NaN would be in every row's sum
-                    _Float16 a, d;
-                    kv_split(ldexpf(x, tex), a, d);
-                    hi[e] = a;
-                    lo[e] = d;
-                }
-                acc[t] = KV_MFMA(hi, ph, acc[t]);
-                acc[t] = KV_MFMA(hi, pl, acc[t]);
-                acc[t] = KV_MFMA(lo, ph, acc[t]);
-            }
-        }
-    }
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
+    const uint64_t place = static_cast<uint64_t>(S.part0) + (unit * A.c.kvh + kvh) * S.splits + split;
+    float* dump = nullptr;   // this lane's row of the unit's scores
+    if (A.scores && m16 < rows) dump = A.scores + (place * A.lines + m16) * 32u * A.per + 32u * wave + 4u * g;
+    KvWave<NT, 1> W;
+    kv_start<NT, 1, CAP>(A, S, kvh, r0, W);
+    kv_run<NT, 1, CAP>(A, S, kvh, sp, pmin, pmax, i0 + wave, i1, 4u, W, dump);
+    float l = add_xor32(add_xor16(W.l[0]));
     if (g == 0u) {
-        s_m[wave][m16] = m;
+        s_m[wave][m16] = W.m[0];
         s_l[wave][m16] = l;
     }
     __syncthreads();
     const float M = fmaxf(fmaxf(s_m[0][m16], s_m[1][m16]), fmaxf(s_m[2][m16], s_m[3][m16]));
     const float ref = M == -INFINITY ? 0.0f : M;
-    float L = 0.0f;
+    const float mine = __builtin_amdgcn_exp2f(W.m[0] - ref);
+    const bool only = S.splits == 1u;
+    for (uint32_t h0 = 0; h0 < rows; h0 += 8u) {
+        if (h0) __syncthreads();
+        if (m16 - h0 < 8u)
 #pragma unroll
-    for (int w = 0; w < 4; ++w) L += s_l[w][m16] * __builtin_amdgcn_exp2f(s_m[w][m16] - ref);
-    const float mine = __builtin_amdgcn_exp2f(m - ref);
+            for (int t = 0; t < 2 * NT; ++t) {
+                f4 v;
 #pragma unroll
-    for (int t = 0; t < 2 * NT; ++t)
+                for (int e = 0; e < 4; ++e) v[e] = ldexpf(W.acc[0][t][e], W.eR - 9) * mine;
+                s_acc[wave][(m16 - h0) * C4 + ((4u * t + g) ^ (m16 & 7u))] = v;   // (rows spread over the banks)
+            }
+        __syncthreads();
+        for (uint32_t u = threadIdx.x; u < min(8u, rows - h0) * C4; u += kKvThreads) {
+            const uint32_t rr = u / C4, c4 = u - rr * C4, row = h0 + rr, at = rr * C4 + (c4 ^ (rr & 7u));
+            const f4 v = (s_acc[0][at] + s_acc[1][at]) + (s_acc[2][at] + s_acc[3][at]);
+            const float m = fmaxf(fmaxf(s_m[0][row], s_m[1][row]), fmaxf(s_m[2][row], s_m[3][row]));
+            const float rf = m == -INFINITY ? 0.0f : m;
+            float L = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[t][e] = ldexpf(acc[t][e], eR - 15) * mine;
-    auto give = [&](uint32_t k) {
+            for (int w = 0; w < 4; ++w) L += s_l[w][row] * __builtin_amdgcn_exp2f(s_m[w][row] - rf);
+            if (only) {
+                const uint32_t r = r0 + row, qi = r / A.G, h = kvh * A.G + (r - qi * A.G);
+                if (4u * c4 < A.c.hd) kv_give(A, S.row0 + qi, h, 4u * c4, v / L);
+                if (c4 == 0u) kv_row_done(A, S.row0 + qi, h, m, L);
+            } else {
+                *reinterpret_cast<f4*>(A.part + (place * A.lines + row) * HDP + 4u * c4) = v;
+            }
+            if (c4 == 0u && (!only || A.scores)) A.part_ml[place * A.lines + row] = make_float2(m, L);
+        }
+    }
+}
+
+// Prompts: a wave per unit of 16 RT rows and split of its blocks; the four waves of a workgroup have neighbouring units of one
+// head and read the same blocks at about the same time. The units of one (head, sequence) are dealt to workgroups that are a
+// multiple of the (head, sequence)s apart, the longest first: with eight of them or a multiple each has an XCD's L2 to itself.
+template <int NT, int RT, bool CAP>
+__global__ void __launch_bounds__(kKvThreads, 2) k_kv8_prompt(const Kv8AttnArgs A) {
+    const uint32_t pairs = A.nseq * A.c.kvh, pair = blockIdx.x % pairs, rest = blockIdx.x / pairs;
+    const uint32_t kvh = pair % A.c.kvh, split = rest % A.splits;
+    const Kv8Seq& S = A.s[pair / A.c.kvh];
+    const uint32_t R = S.n * A.G, U = 16u * RT, units = (R + U - 1u) / U, group = rest / A.splits;
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, m16 = lane & 15u;
+    if (4u * group + wave >= units || split >= S.splits) return;   // whole waves: no barrier follows
+    const uint32_t unit = units - 1u - (4u * group + wave), r0 = U * unit;
+    const uint32_t pmin = S.pos + r0 / A.G, pmax = S.pos + min(r0 + U - 1u, R - 1u) / A.G;
+    const KvSpan sp = kv_span(A, S, pmin, pmax);
+    const uint32_t i0 = split * A.per, i1 = min(sp.n, i0 + A.per);
+    if (i0 >= i1) return;
+    KvWave<NT, RT> W;
+    kv_start<NT, RT, CAP>(A, S, kvh, r0, W);
+    kv_run<NT, RT, CAP>(A, S, kvh, sp, pmin, pmax, i0, i1, 1u, W, nullptr);
+    const bool only = sp.n <= A.per;
+    const uint64_t place = static_cast<uint64_t>(S.part0) + (unit * A.c.kvh + kvh) * S.splits + split;
 #pragma unroll
-        for (int t = 0; t < 2 * NT; ++t) *reinterpret_cast<f4*>(&s_acc[k][m16 * kRow + 16u * t + 4u * g]) = acc[t];
-    };
-    auto take = [&](uint32_t k) {
+    for (int k = 0; k < RT; ++k) {
+        const uint32_t rr = 16u * k + m16, r = r0 + rr;
+        const float L = add_xor32(add_xor16(W.l[k]));
+        if (r >= R) continue;
+        if (only) {
+            const uint32_t qi = r / A.G, h = kvh * A.G + (r - qi * A.G);
+            const float inv = 1.0f / L;
 #pragma unroll
-        for (int t = 0; t < 2 * NT; ++t) acc[t] += *reinterpret_cast<const f4*>(&s_acc[k][m16 * kRow + 16u * t + 4u * g]);
-    };
-    if (wave >= 2u) give(wave - 2u);
-    __syncthreads();
-    if (wave < 2u) take(wave);
-    __syncthreads();
-    if (wave == 1u) give(0u);
-    __syncthreads();
-    if (wave != 0u) return;
-    take(0u);
-    const uint32_t r = r0 + m16;
-    if (sp.n <= A.per) {   // the only split
+            for (int t = 0; t < 2 * NT; ++t) {
+                f4 v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = ldexpf(W.acc[k][t][e], W.eR - 9) * inv;
+                if (16u * t + 4u * g < A.c.hd) kv_give(A, S.row0 + qi, h, 16u * t + 4u * g, v);
+            }
+            if (g == 0u) kv_row_done(A, S.row0 + qi, h, W.m[k], L);
+        } else {
+#pragma unroll
+            for (int t = 0; t < 2 * NT; ++t) {
+                f4 v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = ldexpf(W.acc[k][t][e], W.eR - 9);
+                *reinterpret_cast<f4*>(A.part + (place * A.lines + rr) * 32u * NT + 16u * t + 4u * g) = v;
+            }
+            if (g == 0u) A.part_ml[place * A.lines + rr] = make_float2(W.m[k], L);
+        }
+    }
+}
+
+// The splits of a row put together, one workgroup per (row, head, sequence): four-dim columns times groups of splits, which
+// meet in LDS. With scores (single tokens): workgroups past the rows take 256 positions each, and add up their weights.
+__global__ void __launch_bounds__(kKvThreads) k_kv8_join(const Kv8AttnArgs A) {
+    __shared__ f4 s_o[kKvThreads];
+    __shared__ float s_l[kKvThreads];
+    __shared__ float s_ref[64], s_inv[64];
+    const Kv8Seq& S = A.s[blockIdx.z];
+    const Kv8Dev& c = A.c;
+    const uint32_t kvh = blockIdx.y, R = S.n * A.G, U = A.unit, tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
+    const uint32_t join_rows = A.splits > 1u ? A.rows_most : 0u;
+    if (blockIdx.x < join_rows) {
+        const uint32_t r = blockIdx.x, unit = r / U, rr = r - unit * U;
         if (r >= R) return;
+        const KvSpan sp = kv_span(A, S, S.pos + unit * U / A.G, S.pos + min(unit * U + U - 1u, R - 1u) / A.G);
+        const uint32_t n = (sp.n + A.per - 1u) / A.per;
+        if (S.splits == 1u || (n <= 1u && A.prompt)) return;   // written by the only split
+        const uint64_t p0 = static_cast<uint64_t>(S.part0) + (unit * c.kvh + kvh) * S.splits;
+        float M = -INFINITY;
+        for (uint32_t k = lane; k < n; k += 64u) M = fmaxf(M, A.part_ml[(p0 + k) * A.lines + rr].x);
+        M = wave_red_max(M);
+        const float ref = M == -INFINITY ? 0.0f : M;
+        const uint32_t hd4 = c.hd >> 2, groups = kKvThreads / hd4, grp = tid / hd4, d = (tid - grp * hd4) * 4u;
+        f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+        float L = 0.0f;
+        if (grp < groups)
+            for (uint32_t k = grp; k < n; k += groups) {
+                const float2 ml = A.part_ml[(p0 + k) * A.lines + rr];
+                const float w = __builtin_amdgcn_exp2f(ml.x - ref);
+                L += w * ml.y;
+                o += w * *reinterpret_cast<const f4*>(A.part + ((p0 + k) * A.lines + rr) * c.hdp + d);
+            }
+        s_o[tid] = o;
+        s_l[tid] = L;
+        __syncthreads();
+        if (tid >= hd4) return;
+        for (uint32_t k = 1; k < groups; ++k) {
+            o += s_o[tid + k * hd4];
+            L += s_l[tid + k * hd4];
+        }
         const uint32_t qi = r / A.G, h = kvh * A.G + (r - qi * A.G);
-#pragma unroll
-        for (int t = 0; t < 2 * NT; ++t)
-            if (16u * t + 4u * g < c.hd) kv_give(A, S.row0 + qi, h, 16u * t + 4u * g, acc[t] / L);
-        if (g == 0u) kv_row_done(A, S.row0 + qi, h, M, L);
+        kv_give(A, S.row0 + qi, h, d, o / L);
+        if (tid == 0u) kv_row_done(A, S.row0 + qi, h, M, L);
         return;
     }
-    if (r >= R) return;
-    const uint64_t pr = (static_cast<uint64_t>(S.part0) + (tile * c.kvh + kvh) * S.splits + split) * 16u + m16;
-#pragma unroll
-    for (int t = 0; t < 2 * NT; ++t) *reinterpret_cast<f4*>(A.part + pr * c.hdp + 16u * t + 4u * g) = acc[t];
-    if (g == 0u) A.part_ml[pr] = make_float2(M, L);
-}
-
-// The splits of a row tile put together: one workgroup per (row tile, head, sequence).
-__global__ void __launch_bounds__(kKvThreads) k_kv8_merge(const Kv8AttnArgs A) {
-    const Kv8Seq& S = A.s[blockIdx.z];
-    const Kv8Dev& c = A.c;
-    const uint32_t kvh = blockIdx.y, tile = blockIdx.x, R = S.n * A.G, r0 = 16u * tile;
-    if (r0 >= R) return;
-    const KvSpan sp = kv_span(A, S, S.pos + r0 / A.G, S.pos + min(r0 + 15u, R - 1u) / A.G);
-    const uint32_t n = (sp.n + A.per - 1u) / A.per;
-    if (n <= 1u) return;   // written by the only split
-    const uint64_t p0 = (static_cast<uint64_t>(S.part0) + (tile * c.kvh + kvh) * S.splits) * 16u;
-    const uint32_t hd4 = c.hd >> 2, rows = min(16u, R - r0);
-    for (uint32_t u = threadIdx.x; u < rows * hd4; u += kKvThreads) {
-        uint32_t rr, d;
-        kv_unit(u, hd4, rr, d);
-        float M = -INFINITY;
-        for (uint32_t k = 0; k < n; ++k) M = fmaxf(M, A.part_ml[p0 + k * 16u + rr].x);
-        const float ref = M == -INFINITY ? 0.0f : M;
-        float L = 0.0f;
-        f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (uint32_t k = 0; k < n; ++k) {
-            const float2 ml = A.part_ml[p0 + k * 16u + rr];
-            const float w = __builtin_amdgcn_exp2f(ml.x - ref);
-            L += w * ml.y;
-            o += w * *reinterpret_cast<const f4*>(A.part + (p0 + k * 16u + rr) * c.hdp + d);
-        }
-        const uint32_t r = r0 + rr, qi = r / A.G, h = kvh * A.G + (r - qi * A.G);
-        kv_give(A, S.row0 + qi, h, d, o / L);
-        if (d == 0u) kv_row_done(A, S.row0 + qi, h, M, L);
-    }
-}
-
-// Accumulated weights: one wave per block of positions; the scores once more, against the rows' final maxima and sums.
-template <int NT, bool CAP>
-__global__ void __launch_bounds__(kKvThreads) k_kv8_weights(const Kv8AttnArgs A) {
-    const Kv8Seq& S = A.s[blockIdx.z];
-    const Kv8Dev& c = A.c;
-    const uint32_t kvh = blockIdx.y, lane = threadIdx.x & 63u, g = lane >> 4, m16 = lane & 15u;
-    const uint32_t len = S.pos + S.n, R = S.n * A.G;
-    const uint32_t b = blockIdx.x * 4u + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (S.n == 0u || 32u * b >= len) return;
-    float w[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    const uint32_t j = (blockIdx.x - join_rows) * kKvThreads + tid, len = S.pos + S.n;
+    if (S.n == 0u || j - tid >= len) return;
+    float w = 0.0f;
     for (uint32_t r0 = 0; r0 < R; r0 += 16u) {
+        const uint32_t unit = r0 / 16u, rows = min(16u, R - r0), pmin = S.pos + r0 / A.G, pmax = S.pos + (r0 + rows - 1u) / A.G;
+        const KvSpan sp = kv_span(A, S, pmin, pmax);
+        const uint64_t p0 = static_cast<uint64_t>(S.part0) + (unit * c.kvh + kvh) * S.splits;
+        const uint32_t n = (sp.n + A.per - 1u) / A.per;
+        __syncthreads();
+        for (uint32_t rr = wave; rr < rows; rr += kKvThreads / 64u) {
+            float M = -INFINITY, L = 0.0f;
+            for (uint32_t k = lane; k < n; k += 64u) M = fmaxf(M, A.part_ml[(p0 + k) * A.lines + rr].x);
+            M = wave_red_max(M);
+            const float ref = M == -INFINITY ? 0.0f : M;
+            for (uint32_t k = lane; k < n; k += 64u) {
+                const float2 ml = A.part_ml[(p0 + k) * A.lines + rr];
+                L += ml.y * __builtin_amdgcn_exp2f(ml.x - ref);
+            }
+            L = wave_sum(L);
+            if (lane == 0u) {
+                s_ref[rr] = ref;
+                s_inv[rr] = 1.0f / L;
+            }
+        }
+        __syncthreads();
+        // position j's virtual block: in the prefix, or from lo on
+        const uint32_t b = j >> 5, i = b < sp.n_pre ? b : b - sp.lo + sp.n_pre;
+        if (j >= len || (b >= sp.n_pre && b < sp.lo) || i >= sp.n) continue;
+        const uint32_t k = i / A.per;
+        const float* src = A.scores + (p0 + k) * A.lines * 32u * A.per + 32u * (i - k * A.per) + (j & 31u);
+        for (uint32_t rr = 0; rr < rows; ++rr) w += __builtin_amdgcn_exp2f(src[rr * 32u * A.per] - s_ref[rr]) * s_inv[rr];
+    }
+    if (j >= len) return;
+    const uint64_t at = (static_cast<uint64_t>(S.seq) * c.kvh + kvh) * A.max_ctx + j;
+    A.w_out[at] = (A.w_in && j < S.pos ? A.w_in[at] : 0.0f) + w;
+}
+
+// Prompts' accumulated weights: one workgroup per (block of positions, head, sequence), its waves taking every fourth tile of 16
+// rows; the scores once more, against the rows' final maxima and sums.
+template <int NT, bool CAP>
+__global__ void __launch_bounds__(kKvThreads, 2) k_kv8_weights(const Kv8AttnArgs A) {
+    __shared__ float s_w[4][32];
+    const Kv8Seq& S = A.s[blockIdx.z];
+    const Kv8Dev& c = A.c;
+    const uint32_t kvh = blockIdx.y, m16 = threadIdx.x & 15u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t len = S.pos + S.n, R = S.n * A.G, b = blockIdx.x;
+    if (S.n == 0u || 32u * b >= len) return;
+    const bool open = (b + 1u) * 32u > len, in_pre = 32u * b < S.prefix;
+    float w[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    float ks[8];
+    KvRaw<NT> K;
+    const uint64_t kb = kv_tail_buf(c, S.seq, kvh, b, 0u);
+    if (open) {
+#pragma unroll
+        for (uint32_t e = 0; e < 8u; ++e) ks[e] = 32u * b + kv_token(e) < len ? c.factor[kb * 32u + kv_token(e)] : 0.0f;
+    } else {
+        const uint64_t blk = kv_block(c, S.seq, kvh, b);
+        kv_load<NT>(c, blk, 0u, K);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ks[e] = c.scales[blk].x;
+    }
+    for (uint32_t r0 = 16u * wave; r0 < R; r0 += 64u) {
         const uint32_t pmin = S.pos + r0 / A.G, pmax = S.pos + min(r0 + 15u, R - 1u) / A.G;
-        const bool in_pre = 32u * b < S.prefix;
         if (!in_pre && 32u * b > pmax) continue;
         if (!in_pre && A.window && pmin >= A.window && 32u * b + 31u <= pmin - A.window) break;   // and no later row sees it
-        KvQuery<NT> Q;
-        kv_load_q<NT>(A, S, kvh, r0, Q);
-        float s[8];
-        kv_scores<NT, CAP>(A, S, kvh, b, Q, true, s);
+        KvWave<NT, 1> W;
+        kv_start<NT, 1, CAP>(A, S, kvh, r0, W);
+        f4 s[1][2];
+        if (open) kv_scores_open<NT, 1>(c, kb, W, s);
+        else kv_scores<NT, 1>(K, W, s);
         const uint32_t r = r0 + m16;
-        if (r < R) {
-            const uint32_t qi = r / A.G, h = kvh * A.G + (r - qi * A.G);
-            const float2 st = A.stats[(static_cast<uint64_t>(S.row0) + qi) * A.heads + h];
+        if (r >= R) continue;
+        const uint32_t qi = r / A.G, h = kvh * A.G + (r - qi * A.G);
+        const float2 st = A.stats[(static_cast<uint64_t>(S.row0) + qi) * A.heads + h];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] += s[e] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s[e] - st.x) * st.y;
+        for (uint32_t e = 0; e < 8u; ++e) {
+            float x = s[0][e >> 2][e & 3u] * (W.f[0] * ks[e]);
+            if constexpr (CAP) x = A.cap * 1.4426950409f * kv_tanh(x * (1.0f / A.cap));
+            const uint32_t j = 32u * b + kv_token(e);
+            const bool y = j < len && (j < S.prefix || (j <= W.p[0] && (!A.window || W.p[0] - j < A.window)));
+            w[e] += y ? __builtin_amdgcn_exp2f(x - st.x) * st.y : 0.0f;
         }
     }
-    const uint64_t base = (static_cast<uint64_t>(S.seq) * c.kvh + kvh) * A.max_ctx;
 #pragma unroll
     for (uint32_t e = 0; e < 8u; ++e) {
         const float t = slot_sum<16>(w[e]);
-        const uint32_t j = 32u * b + 4u * g + (e & 3u) + 16u * (e >> 2);
-        if (m16 == 0u && j < len) A.w_out[base + j] = (A.w_in && j < S.pos ? A.w_in[base + j] : 0.0f) + t;
+        if (m16 == 0u) s_w[wave][kv_token(e)] = t;
     }
+    __syncthreads();
+    const uint32_t j = 32u * b + threadIdx.x;
+    if (threadIdx.x >= 32u || j >= len) return;
+    const float t = (s_w[0][threadIdx.x] + s_w[1][threadIdx.x]) + (s_w[2][threadIdx.x] + s_w[3][threadIdx.x]);
+    const uint64_t at = (static_cast<uint64_t>(S.seq) * c.kvh + kvh) * A.max_ctx + j;
+    A.w_out[at] = (A.w_in && j < S.pos ? A.w_in[at] : 0.0f) + t;
 }
 
 // ---- eviction -------------------------------------------------------------------------------
@@ -725,6 +1004,7 @@ __global__ void __launch_bounds__(kKvThreads) k_kv8_gather(const Kv8EvictArgs A)
     const bool closed = (b + 1u) * 32u <= V.keep, tail = b + 1u >= (V.keep - 1u) >> 5;   // the last block and the one before
     KvTile T;
     const uint32_t hd4 = c.hd >> 2, units = 32u * hd4;
+    const uint64_t buf = kv_tail_buf(c, V.dst, head, b, z);
 #pragma unroll
     for (uint32_t k = 0; k < 8u; ++k) {
         const uint32_t u = tid + kKvThreads * k;
@@ -736,19 +1016,16 @@ __global__ void __launch_bounds__(kKvThreads) k_kv8_gather(const Kv8EvictArgs A)
         const uint32_t p = kept[32u * b + t];
 #pragma unroll
         for (uint32_t e = 0; e < 4u; ++e) T.v[k][e] = kv_value(c, V.src, head, z, p, d + e, V.len);
-        if (tail) *reinterpret_cast<f4*>(c.tail + kv_tail_row(c, V.dst, head, b, z, t) * c.hdp + d) = T.v[k];
+        if (tail) *reinterpret_cast<f4*>(c.tail + (buf * 32u + t) * c.hdp + d) = T.v[k];
     }
     if (closed) kv_close_block(c, T, kv_block(c, V.dst, head, b), z, img, red);
     if (!tail) return;
-    __syncthreads();   // the tail rows are whole: their maxima, and zeros in the padding dimensions
+    __syncthreads();   // the tail's rows are whole: a wave each for their pairs
     const uint32_t n = min(32u, V.keep - 32u * b), lane = tid & 63u;
     for (uint32_t t = tid >> 6; t < n; t += kKvThreads / 64u) {
-        const uint64_t row = kv_tail_row(c, V.dst, head, b, z, t);
         f4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (4u * lane < c.hd) v = *reinterpret_cast<const f4*>(c.tail + row * c.hdp + 4u * lane);
-        else if (4u * lane < c.hdp) *reinterpret_cast<f4*>(c.tail + row * c.hdp + 4u * lane) = v;
-        const uint32_t m = wave_max_u32(max(max(f_bits(v[0]), f_bits(v[1])), max(f_bits(v[2]), f_bits(v[3]))));
-        if (lane == 0u) c.tmax[row] = __uint_as_float(m);
+        if (4u * lane < c.hd) v = *reinterpret_cast<const f4*>(c.tail + (buf * 32u + t) * c.hdp + 4u * lane);
+        kv_store_tail(c, buf, z, t, v, false);
     }
 }
 
@@ -822,12 +1099,12 @@ int check_array(const void* p, uint64_t* stride, uint64_t width, const char* who
 // Blocks that a span of positions touches.
 uint32_t touched(const Kv8Seq& s) { return s.n ? ((s.pos + s.n - 1u) >> 5) - (s.pos >> 5) + 1u : 0u; }
 
-// The most blocks that a row tile of a sequence sees.
-uint32_t most_blocks(const Kv8Seq& s, uint32_t window) {
+// The most blocks that a unit's rows of a sequence see.
+uint32_t most_blocks(const Kv8Seq& s, uint32_t window, uint32_t unit) {
     const uint32_t len = s.pos + s.n, pre = std::min(s.prefix, len), all = (len + 31u) / 32u;
     if (!window) return all;
-    // a tile's rows span 16 positions at most
-    const uint64_t w = static_cast<uint64_t>((pre + 31u) / 32u) + (static_cast<uint64_t>(window) + 15u + 31u) / 32u + 1u;
+    // (its rows span that many positions at most)
+    const uint64_t w = static_cast<uint64_t>((pre + 31u) / 32u) + (static_cast<uint64_t>(window) + unit + 31u) / 32u + 1u;
     return static_cast<uint32_t>(std::min<uint64_t>(all, w));
 }
 
@@ -858,35 +1135,32 @@ int attn_plan(const vrt_kv8_cache* c, const vrt_kv8_attn* at, const vrt_kv8_rows
         VRT_REQUIRE(!scored || len <= c->max_ctx, "%s: weights need pos + n <= max_ctx", who);
         items += (static_cast<uint64_t>(s.n) * A.G + 15u) / 16u * c->kv_heads;
     }
-    VRT_REQUIRE(*total * A.G <= 0x3fffffffu && items <= 0x3fffffffu, "%s: too many rows", who);
+    VRT_REQUIRE(*total * A.G <= 0x3fffffffu && items <= 0x3fffffu, "%s: too many rows", who);   // grids of 2^31 workgroups
     *P = kv8_plan(A, c->kv_heads, z.hdp, n, *total, scored);
     return VRT_OK;
 }
 
-template <bool CAP>
-const void* attn_kernel(uint32_t nt) {
-    switch (nt) {
-        case 1: return reinterpret_cast<const void*>(&k_kv8_attn<1, CAP>);
-        case 2: return reinterpret_cast<const void*>(&k_kv8_attn<2, CAP>);
-        case 3: return reinterpret_cast<const void*>(&k_kv8_attn<3, CAP>);
-        case 4: return reinterpret_cast<const void*>(&k_kv8_attn<4, CAP>);
-        case 5: return reinterpret_cast<const void*>(&k_kv8_attn<5, CAP>);
-        case 6: return reinterpret_cast<const void*>(&k_kv8_attn<6, CAP>);
-        case 7: return reinterpret_cast<const void*>(&k_kv8_attn<7, CAP>);
-        default: return reinterpret_cast<const void*>(&k_kv8_attn<8, CAP>);
-    }
+// Tiles of 16 rows that a prompt's wave runs together: as many as leave two waves a SIMD.
+constexpr int rows_of(int nt) { return nt <= 4 ? 2 : 1; }
+
+template <int NT>
+const void* attn_kernel(bool cap, int which) {   // 0 single tokens, 1 prompts, 2 prompts' weights
+    constexpr int RT = rows_of(NT);
+    if (which == 0) return cap ? reinterpret_cast<const void*>(&k_kv8_attn<NT, true>) : reinterpret_cast<const void*>(&k_kv8_attn<NT, false>);
+    if (which == 1)
+        return cap ? reinterpret_cast<const void*>(&k_kv8_prompt<NT, RT, true>) : reinterpret_cast<const void*>(&k_kv8_prompt<NT, RT, false>);
+    return cap ? reinterpret_cast<const void*>(&k_kv8_weights<NT, true>) : reinterpret_cast<const void*>(&k_kv8_weights<NT, false>);
 }
-template <bool CAP>
-const void* weights_kernel(uint32_t nt) {
+const void* attn_kernel(uint32_t nt, bool cap, int which) {
     switch (nt) {
-        case 1: return reinterpret_cast<const void*>(&k_kv8_weights<1, CAP>);
-        case 2: return reinterpret_cast<const void*>(&k_kv8_weights<2, CAP>);
-        case 3: return reinterpret_cast<const void*>(&k_kv8_weights<3, CAP>);
-        case 4: return reinterpret_cast<const void*>(&k_kv8_weights<4, CAP>);
-        case 5: return reinterpret_cast<const void*>(&k_kv8_weights<5, CAP>);
-        case 6: return reinterpret_cast<const void*>(&k_kv8_weights<6, CAP>);
-        case 7: return reinterpret_cast<const void*>(&k_kv8_weights<7, CAP>);
-        default: return reinterpret_cast<const void*>(&k_kv8_weights<8, CAP>);
+        case 1: return attn_kernel<1>(cap, which);
+        case 2: return attn_kernel<2>(cap, which);
+        case 3: return attn_kernel<3>(cap, which);
+        case 4: return attn_kernel<4>(cap, which);
+        case 5: return attn_kernel<5>(cap, which);
+        case 6: return attn_kernel<6>(cap, which);
+        case 7: return attn_kernel<7>(cap, which);
+        default: return attn_kernel<8>(cap, which);
     }
 }
 
@@ -907,8 +1181,9 @@ Kv8Sizes kv8_sizes(uint32_t max_seqs, uint32_t max_ctx, uint32_t kv_heads, uint3
     z.codes = up256(blocks * 64u * z.hdp);
     z.scales = up256(blocks * sizeof(float2));
     z.tail = up256(heads * 128u * z.hdp * 4u);
-    z.tmax = up256(heads * 128u * 4u);
-    z.total = z.codes + z.scales + z.tail + z.tmax;
+    z.pairs = up256(heads * 256u * z.hdp * 2u);
+    z.factor = up256(heads * 128u * 4u);
+    z.total = z.codes + z.scales + z.tail + z.pairs + z.factor;
     return z;
 }
 
@@ -918,7 +1193,8 @@ Kv8Dev kv8_view(const Kv8Sizes& z, void* data, uint32_t kv_heads, uint32_t head_
     d.codes = p;
     d.scales = reinterpret_cast<float2*>(p + z.codes);
     d.tail = reinterpret_cast<float*>(p + z.codes + z.scales);
-    d.tmax = reinterpret_cast<float*>(p + z.codes + z.scales + z.tail);
+    d.pairs = reinterpret_cast<_Float16*>(p + z.codes + z.scales + z.tail);
+    d.factor = reinterpret_cast<float*>(p + z.codes + z.scales + z.tail + z.pairs);
     d.nb = z.nb;
     d.kvh = kv_heads;
     d.hd = head_dim;
@@ -926,38 +1202,57 @@ Kv8Dev kv8_view(const Kv8Sizes& z, void* data, uint32_t kv_heads, uint32_t head_
     return d;
 }
 
-// About kKvSplits workgroups, of four blocks at least.
-constexpr uint64_t kKvSplits = 1024;
+// Single tokens: about 512 workgroups, two a CU, of four blocks at least. Prompts: about 1536 waves' worth of blocks, 16 at least.
+constexpr uint64_t kKvSplits = 512, kKvPromptSplits = 1536;
 
 Kv8Plan kv8_plan(Kv8AttnArgs& A, uint32_t kvh, uint32_t hdp, uint32_t n, uint64_t rows, bool scored) {
     Kv8Plan P{};
-    uint64_t blocks = 0;   // of all row tiles and heads
-    for (uint32_t i = 0; i < n; ++i)
-        blocks += static_cast<uint64_t>((A.s[i].n * A.G + 15u) / 16u) * kvh * most_blocks(A.s[i], A.window);
-    const uint64_t per = std::max<uint64_t>(4u, (blocks + kKvSplits - 1u) / kKvSplits);
+    uint32_t active = 0;
+    A.rows_most = 0;
+    for (uint32_t i = 0; i < n; ++i) {
+        active += A.s[i].n != 0u;
+        A.rows_most = std::max(A.rows_most, A.s[i].n * A.G);
+    }
+    A.nseq = n;
+    A.prompt = rows * A.G > 32ull * active;
+    A.unit = A.prompt ? 16u * rows_of(static_cast<int>(hdp / 32u)) : 16u;
+    A.lines = std::min(A.unit, std::max(1u, A.rows_most));
+    uint64_t blocks = 0;   // of all units and heads; a prompt's queries see half of its own on average
+    for (uint32_t i = 0; i < n; ++i) {
+        const Kv8Seq& s = A.s[i];
+        const uint32_t most = most_blocks(s, A.window, A.unit);
+        blocks += static_cast<uint64_t>((s.n * A.G + A.unit - 1u) / A.unit) * kvh *
+                  (s.prefix ? most : std::min(most, (s.pos + (s.n + 1u) / 2u + 31u) / 32u));
+    }
+    const uint64_t per = A.prompt ? std::max<uint64_t>(16u, (blocks + kKvPromptSplits - 1u) / kKvPromptSplits)
+                                  : std::max<uint64_t>(4u, (blocks + kKvSplits - 1u) / kKvSplits);
     A.per = static_cast<uint32_t>((per + 3u) & ~3ull);
     A.splits = 1u;
+    const bool dump = scored && !A.prompt;
     uint64_t place = 0;
     for (uint32_t i = 0; i < n; ++i) {
         Kv8Seq& s = A.s[i];
-        const uint32_t tiles = (s.n * A.G + 15u) / 16u;
-        s.splits = std::max(1u, (most_blocks(s, A.window) + A.per - 1u) / A.per);
+        const uint32_t units = (s.n * A.G + A.unit - 1u) / A.unit;
+        s.splits = std::max(1u, (most_blocks(s, A.window, A.unit) + A.per - 1u) / A.per);
         s.part0 = static_cast<uint32_t>(place);
-        if (s.splits > 1u) place += static_cast<uint64_t>(tiles) * kvh * s.splits;
+        if (s.splits > 1u || dump) place += static_cast<uint64_t>(units) * kvh * s.splits;
         A.splits = std::max(A.splits, s.splits);
-        P.tiles = std::max(P.tiles, tiles);
+        P.units = std::max(P.units, units);
     }
-    P.part = up256(place * 16u * hdp * 4u);
-    P.ml = up256(place * 16u * sizeof(float2));
-    P.stats = scored ? up256(rows * A.heads * sizeof(float2)) : 0u;
-    P.total = P.part + P.ml + P.stats;
+    P.part = A.splits > 1u ? up256(place * A.lines * hdp * 4u) : 0u;
+    P.ml = up256(place * A.lines * sizeof(float2));
+    P.extra = !scored ? 0u : dump ? up256(place * A.lines * 32u * A.per * 4u) : up256(rows * A.heads * sizeof(float2));
+    P.total = P.part + P.ml + P.extra;
     return P;
 }
 
-// (a sequence's splits are at most its blocks / per + 1, and all blocks / per at most kKvSplits)
-uint64_t kv8_workspace_most(uint64_t items, uint32_t hdp, uint64_t rows, uint32_t heads) {
-    const uint64_t place = kKvSplits + items;
-    return up256(place * 16u * hdp * 4u) + up256(place * 16u * sizeof(float2)) + up256(rows * heads * sizeof(float2));
+// Blocks a sequence's unit and head: at most ceil(max_ctx / 32); splits: at most blocks / per + 1, all blocks / per at most kKvSplits.
+uint64_t kv8_workspace_most(uint32_t seqs, uint32_t max_ctx, uint32_t heads, uint32_t kvh, uint32_t hdp, bool scored) {
+    const uint64_t items = static_cast<uint64_t>(seqs) * kvh * ((heads / kvh + 15u) / 16u), blocks = items * ((max_ctx + 31u) / 32u);
+    const uint64_t per = (std::max<uint64_t>(4u, (blocks + kKvSplits - 1u) / kKvSplits) + 3u) & ~3ull;
+    const uint64_t place = kKvSplits + items, lines = std::min(16u, heads / kvh);
+    return up256(place * lines * hdp * 4u) + up256(place * lines * sizeof(float2)) +
+           (scored ? up256((blocks + items * per) * lines * 32u * 4u) : 0u);
 }
 
 int kv8_append(const Kv8Dev& c, const Kv8Seq* seqs, uint32_t n, const float* k, const float* v, uint64_t stride, hipStream_t s) {
@@ -977,20 +1272,23 @@ int kv8_append(const Kv8Dev& c, const Kv8Seq* seqs, uint32_t n, const float* k, 
 
 int kv8_attend(Kv8AttnArgs& A, const Kv8Plan& P, void* workspace, uint32_t n, hipStream_t s) {
     auto* ws = static_cast<uint8_t*>(workspace);
+    const bool scored = A.w_out != nullptr, cap = A.cap > 0.0f;
     A.part = reinterpret_cast<float*>(ws);
     A.part_ml = reinterpret_cast<float2*>(ws + P.part);
-    A.stats = A.w_out ? reinterpret_cast<float2*>(ws + P.part + P.ml) : nullptr;
+    auto* extra = reinterpret_cast<float*>(ws + P.part + P.ml);
+    A.scores = scored && !A.prompt ? extra : nullptr;
+    A.stats = scored && A.prompt ? reinterpret_cast<float2*>(extra) : nullptr;
     const uint32_t nt = A.c.hdp / 32u;
-    const bool cap = A.cap > 0.0f;
-    if (int rc = launch(cap ? attn_kernel<true>(nt) : attn_kernel<false>(nt), dim3(P.tiles * A.splits, A.c.kvh, n), kKvThreads, A, s))
-        return rc;
-    if (A.splits > 1u)
-        if (int rc = launch(reinterpret_cast<const void*>(&k_kv8_merge), dim3(P.tiles, A.c.kvh, n), kKvThreads, A, s)) return rc;
-    if (!A.w_out) return VRT_OK;
+    const dim3 grid = A.prompt ? dim3((P.units + 3u) / 4u * A.splits * A.c.kvh * n) : dim3(P.units * A.splits, A.c.kvh, n);
+    if (int rc = launch(attn_kernel(nt, cap, A.prompt ? 1 : 0), grid, kKvThreads, A, s)) return rc;
     uint32_t len = 0;
     for (uint32_t i = 0; i < n; ++i)
         if (A.s[i].n) len = std::max(len, A.s[i].pos + A.s[i].n);
-    return launch(cap ? weights_kernel<true>(nt) : weights_kernel<false>(nt), dim3((len + 127u) / 128u, A.c.kvh, n), kKvThreads, A, s);
+    const uint32_t wgs = (A.splits > 1u ? A.rows_most : 0u) + (A.scores ? (len + kKvThreads - 1u) / kKvThreads : 0u);
+    if (wgs)
+        if (int rc = launch(reinterpret_cast<const void*>(&k_kv8_join), dim3(wgs, A.c.kvh, n), kKvThreads, A, s)) return rc;
+    if (!scored || !A.prompt) return VRT_OK;
+    return launch(attn_kernel(nt, cap, 2), dim3((len + 31u) / 32u, A.c.kvh, n), kKvThreads, A, s);
 }
 
 int kv8_evict(const Kv8Dev& c, const vrt_kv8_move* moves, uint32_t n, float* weights, uint32_t max_ctx, uint32_t* kept,
