@@ -37,9 +37,18 @@ __device__ __forceinline__ uint32_t kv_v_at(uint32_t t, uint32_t d) {
     return (d >> 5) * 1024u + (((t >> 2) & 3u) * 16u + (d & 15u)) * 16u + ((d >> 4) & 1u) * 8u + (t & 3u) + (t >> 4) * 4u;
 }
 
-__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
-    for (int o = 32; o > 0; o >>= 1) v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), o)));
-    return v;
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_max_u32(uint32_t v) {   // lanes outside the row mask keep their own
+    return max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(static_cast<int>(v), static_cast<int>(v), CTRL, ROWS, 0xf, false)));
+}
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {   // wave-uniform (the steps of wave_red_max)
+    v = dpp_max_u32<0xB1, 0xf>(v);
+    v = dpp_max_u32<0x4E, 0xf>(v);
+    v = dpp_max_u32<0x141, 0xf>(v);
+    v = dpp_max_u32<0x140, 0xf>(v);
+    v = dpp_max_u32<0x142, 0xa>(v);
+    v = dpp_max_u32<0x143, 0xc>(v);
+    return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), 63));
 }
 
 // x = hi + lo in f16 (x below 2^15 in magnitude; what is lost is below 2^-24)
@@ -59,69 +68,81 @@ __device__ __forceinline__ float kv_round(float x, float s, float inv) {
 #pragma clang fp contract(off)
     float q = rintf(x * inv);
     const float r = __builtin_fmaf(-q, s, x), half = 0.5f * s;
-    if (fabsf(r) >= half) {   // seldom
-        const bool odd = static_cast<int>(q) & 1;
-        if (r > half || (r == half && odd)) q += 1.0f;
-        else if (r < -half || (r == -half && odd)) q -= 1.0f;
-    }
-    return fminf(fmaxf(q, -127.0f), 127.0f);
+    const bool odd = static_cast<int>(q) & 1;
+    if (r > half || (r == half && odd)) q += 1.0f;
+    else if (r < -half || (r == -half && odd)) q -= 1.0f;
+    return __builtin_amdgcn_fmed3f(q, -127.0f, 127.0f);
 }
 
 // ---- append ---------------------------------------------------------------------------------
 
-// A workgroup's 32 x hd values of one head and block, as up to 8 float4 per thread (unit tid + 256 k: token
-// unit / (hd / 4), dims 4 (unit % (hd / 4)) ..): amax, scale, codes, in operand order through an LDS image.
+// A workgroup's 32 rows of one head and block: NT float4 a thread (unit tid + 256 k: token unit / (8 NT), dims 4 (unit %
+// (8 NT)) ..; zeros past hd), their largest magnitude, scale, codes, in operand order through an LDS image.
+template <int NT>
 struct KvTile {
-    f4 v[8];
+    f4 v[NT];
 };
-// (u / hd4 by a reciprocal: u below 2048, hd4 at most 64)
-__device__ __forceinline__ void kv_unit(uint32_t u, uint32_t hd4, uint32_t& t, uint32_t& d) {
-    t = (u * ((1u << 20) / hd4 + 1u)) >> 20;
-    d = (u - t * hd4) * 4u;
+template <int NT>
+__device__ __forceinline__ void kv_unit(uint32_t k, uint32_t& t, uint32_t& d) {
+    const uint32_t u = threadIdx.x + kKvThreads * k;
+    t = u / (8u * NT);
+    d = (u - t * 8u * NT) * 4u;
 }
 __device__ __forceinline__ uint32_t f_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-__device__ __forceinline__ void kv_close_block(const Kv8Dev& c, const KvTile& x, uint64_t block, uint32_t z, uint8_t* img,
+template <int NT>
+__device__ __forceinline__ void kv_close_block(const Kv8Dev& c, const KvTile<NT>& x, uint64_t block, uint32_t z, uint8_t* img,
                                                uint32_t* red) {
-    const uint32_t tid = threadIdx.x, hd4 = c.hd >> 2, units = 32u * hd4;
+    const uint32_t tid = threadIdx.x;
     uint32_t m = 0u;   // |x| as integers: larger is larger, NaN above infinity above the rest
 #pragma unroll
-    for (uint32_t k = 0; k < 8u; ++k)
-        if (tid + kKvThreads * k < units)
+    for (int k = 0; k < NT; ++k)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) m = max(m, f_bits(x.v[k][e]));
+        for (int e = 0; e < 4; ++e) m = max(m, f_bits(x.v[k][e]));
     m = wave_max_u32(m);
     if ((tid & 63u) == 0u) red[tid >> 6] = m;
-    if (c.hd != c.hdp)   // the padding dimensions' codes: zeros
-        for (uint32_t i = tid; i < 8u * c.hdp; i += kKvThreads) reinterpret_cast<uint32_t*>(img)[i] = 0x80808080u;
     __syncthreads();
     m = max(max(red[0], red[1]), max(red[2], red[3]));
     const float s = m >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __uint_as_float(m) / 127.0f;
-    const bool live = s > 0.0f;
-    // the quotient's steps stay away from denormals: their halves and reciprocals are no numbers
-    const float up = s < 0x1p-100f ? 0x1p60f : 1.0f, su = s * up;
-    const float inv = live ? 1.0f / su : 0.0f;
+    uint32_t w[NT];
 #pragma unroll
-    for (uint32_t k = 0; k < 8u; ++k) {
-        const uint32_t u = tid + kKvThreads * k;
-        if (u >= units) break;
-        uint32_t t, d, w = 0u;
-        kv_unit(u, hd4, t, d);
+    for (int k = 0; k < NT; ++k) w[k] = 0x80808080u;
+    if (s > 0.0f) {
+        // the quotient's steps stay away from denormals: their halves and reciprocals are no numbers
+        const float up = s < 0x1p-100f ? 0x1p60f : 1.0f, su = s * up, inv = 1.0f / su, half = 0.5f * su;
+        bool near = false;   // a remainder of half a step or more: the quotient may be one off, or a tie
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float q = live ? kv_round(x.v[k][e] * up, su, inv) : 0.0f;
-            w |= static_cast<uint32_t>(static_cast<int>(q) + 128) << (8 * e);
+        for (int k = 0; k < NT; ++k) {
+            w[k] = 0u;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float y = x.v[k][e] * up, q = __builtin_amdgcn_fmed3f(rintf(y * inv), -127.0f, 127.0f);
+                near |= fabsf(__builtin_fmaf(-q, su, y)) >= half;
+                w[k] = __builtin_amdgcn_cvt_pk_u8_f32(q + 128.0f, e, w[k]);
+            }
         }
+        if (__any(near))   // seldom
+#pragma unroll
+            for (int k = 0; k < NT; ++k) {
+                w[k] = 0u;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[k] = __builtin_amdgcn_cvt_pk_u8_f32(kv_round(x.v[k][e] * up, su, inv) + 128.0f, e, w[k]);
+            }
+    }
+#pragma unroll
+    for (int k = 0; k < NT; ++k) {
+        uint32_t t, d;
+        kv_unit<NT>(k, t, d);
         if (z == 0u) {
-            *reinterpret_cast<uint32_t*>(img + kv_k_at(t, d)) = w;
+            *reinterpret_cast<uint32_t*>(img + kv_k_at(t, d)) = w[k];
         } else {
 #pragma unroll
-            for (uint32_t e = 0; e < 4u; ++e) img[kv_v_at(t, d + e)] = static_cast<uint8_t>(w >> (8u * e));
+            for (uint32_t e = 0; e < 4u; ++e) img[kv_v_at(t, d + e)] = static_cast<uint8_t>(w[k] >> (8u * e));
         }
     }
     __syncthreads();
     uint4* dst = reinterpret_cast<uint4*>(kv_codes(c, block) + z * 32u * c.hdp);
-    for (uint32_t i = tid; i < 2u * c.hdp; i += kKvThreads) dst[i] = reinterpret_cast<const uint4*>(img)[i];
+    for (uint32_t i = tid; i < 64u * NT; i += kKvThreads) dst[i] = reinterpret_cast<const uint4*>(img)[i];
     if (tid == 0u) reinterpret_cast<float*>(c.scales + block)[z] = s;
 }
 
@@ -167,9 +188,9 @@ __device__ __forceinline__ void kv_to_tail(const Kv8Dev& c, uint32_t seq, uint32
     f4 v[8];
 #pragma unroll
     for (uint32_t k = 0; k < 8u; ++k) {
-        const uint32_t p = first + wave + 4u * k;
-        v[k] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-        if (p <= last && 4u * lane < c.hd) v[k] = *reinterpret_cast<const f4*>(x + static_cast<uint64_t>(p - p0) * stride + 4u * lane);
+        const uint32_t p = min(first + wave + 4u * k, last);
+        v[k] = *reinterpret_cast<const f4*>(x + static_cast<uint64_t>(p - p0) * stride + min(4u * lane, c.hd - 4u));
+        if (4u * lane >= c.hd) v[k] = f4{0.0f, 0.0f, 0.0f, 0.0f};
     }
     const uint64_t buf = kv_tail_buf(c, seq, head, b, z);
 #pragma unroll
@@ -187,32 +208,29 @@ struct Kv8AppendArgs {
 // One workgroup per (block the call touches, head and K or V, sequence). A full block's codes; the rows of the last two
 // blocks also go to the tail. The first block's earlier rows come from the tail, which a later block of the same parity
 // overwrites: the first block's workgroup writes that one's rows too, after it has read its own.
+template <int NT>
 __global__ void __launch_bounds__(kKvThreads) k_kv8_append(const Kv8AppendArgs A) {
-    __shared__ __align__(16) uint8_t img[32 * 256];
+    __shared__ __align__(16) uint8_t img[1024 * NT];
     __shared__ uint32_t red[4];
     const Kv8Dev& c = A.c;
     const Kv8Seq& S = A.s[blockIdx.z];
-    const uint32_t head = blockIdx.y >> 1, z = blockIdx.y & 1u, tid = threadIdx.x;
+    const uint32_t head = blockIdx.y >> 1, z = blockIdx.y & 1u;
     if (S.n == 0u) return;
     const uint32_t end = S.pos + S.n, b0 = S.pos >> 5, bl = (end - 1u) >> 5, b = b0 + blockIdx.x;
     if (b > bl) return;
-    const bool closed = (b + 1u) * 32u <= end;
     const float* x = A.x[z] + static_cast<uint64_t>(S.row0) * A.stride + head * c.hd;
-    if (closed) {
-        KvTile T;
-        const uint32_t hd4 = c.hd >> 2, units = 32u * hd4;
+    if ((b + 1u) * 32u <= end) {
+        KvTile<NT> T;
         const float* old = c.tail + kv_tail_buf(c, S.seq, head, b, z) * 32u * c.hdp;
 #pragma unroll
-        for (uint32_t k = 0; k < 8u; ++k) {
-            const uint32_t u = tid + kKvThreads * k;
-            T.v[k] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-            if (u >= units) continue;
+        for (int k = 0; k < NT; ++k) {
             uint32_t t, d;
-            kv_unit(u, hd4, t, d);
-            const uint32_t p = 32u * b + t;
-            T.v[k] = *reinterpret_cast<const f4*>(p < S.pos ? old + t * c.hdp + d : x + static_cast<uint64_t>(p - S.pos) * A.stride + d);
+            kv_unit<NT>(k, t, d);
+            const uint32_t p = 32u * b + t, dd = min(d, c.hd - 4u);
+            T.v[k] = *reinterpret_cast<const f4*>(p < S.pos ? old + t * c.hdp + dd : x + static_cast<uint64_t>(p - S.pos) * A.stride + dd);
+            if (d >= c.hd) T.v[k] = f4{0.0f, 0.0f, 0.0f, 0.0f};
         }
-        kv_close_block(c, T, kv_block(c, S.seq, head, b), z, img, red);   // (its barriers come after every read of the tail)
+        kv_close_block<NT>(c, T, kv_block(c, S.seq, head, b), z, img, red);   // (its barriers come after every read of the tail)
     }
     const bool shared = (S.pos & 31u) != 0u;   // the first block reads its tail
     for (uint32_t t = bl > b0 ? bl - 1u : bl; t <= bl; ++t) {
@@ -231,25 +249,15 @@ struct Kv8ReadArgs {
     Kv8Seq s[kKvMaxSeqs];   // prefix: the sequence's length
 };
 
-__device__ __forceinline__ float kv_value(const Kv8Dev& c, uint32_t seq, uint32_t head, uint32_t z, uint32_t p, uint32_t d,
-                                          uint32_t len) {
-#pragma clang fp contract(off)
-    const uint32_t b = p >> 5, t = p & 31u;
-    if ((b + 1u) * 32u > len) return c.tail[(kv_tail_buf(c, seq, head, b, z) * 32u + t) * c.hdp + d];
-    const uint64_t blk = kv_block(c, seq, head, b);
-    const uint8_t u = kv_codes(c, blk)[z * 32u * c.hdp + (z ? kv_v_at(t, d) : kv_k_at(t, d))];
-    const float s = reinterpret_cast<const float*>(c.scales + blk)[z];
-    return s * static_cast<float>(static_cast<int>(u) - 128);
-}
-
 // One workgroup per (block, head and K or V, sequence): the block's codes in 16-byte units into LDS, rows out of it.
+template <int NT>
 __global__ void __launch_bounds__(kKvThreads) k_kv8_read(const Kv8ReadArgs A) {
 #pragma clang fp contract(off)
-    __shared__ __align__(16) uint8_t img[32 * 256];
+    __shared__ __align__(16) uint8_t img[1024 * NT];
     const Kv8Dev& c = A.c;
     const Kv8Seq& S = A.s[blockIdx.z];
     const uint32_t head = blockIdx.y >> 1, z = blockIdx.y & 1u, tid = threadIdx.x;
-    const uint32_t b = (S.pos >> 5) + blockIdx.x, hd4 = c.hd >> 2;
+    const uint32_t b = (S.pos >> 5) + blockIdx.x;
     if (S.n == 0u || b > (S.pos + S.n - 1u) >> 5) return;
     const bool closed = (b + 1u) * 32u <= S.prefix;
     float s = 0.0f;
@@ -257,22 +265,23 @@ __global__ void __launch_bounds__(kKvThreads) k_kv8_read(const Kv8ReadArgs A) {
         const uint64_t blk = kv_block(c, S.seq, head, b);
         const uint4* src = reinterpret_cast<const uint4*>(kv_codes(c, blk) + z * 32u * c.hdp);
         s = reinterpret_cast<const float*>(c.scales + blk)[z];
-        for (uint32_t i = tid; i < 2u * c.hdp; i += kKvThreads) reinterpret_cast<uint4*>(img)[i] = src[i];
+        for (uint32_t i = tid; i < 64u * NT; i += kKvThreads) reinterpret_cast<uint4*>(img)[i] = src[i];
         __syncthreads();
     }
     const float* old = c.tail + kv_tail_buf(c, S.seq, head, b, z) * 32u * c.hdp;
-    for (uint32_t u = tid; u < 32u * hd4; u += kKvThreads) {
+#pragma unroll
+    for (int k = 0; k < NT; ++k) {
         uint32_t t, d;
-        kv_unit(u, hd4, t, d);
+        kv_unit<NT>(k, t, d);
         const uint32_t p = 32u * b + t;
-        if (p < S.pos || p - S.pos >= S.n) continue;
+        if (d >= c.hd || p < S.pos || p - S.pos >= S.n) continue;
         f4 v;
         if (closed) {
             uint32_t w;
             if (z == 0u) w = *reinterpret_cast<const uint32_t*>(img + kv_k_at(t, d));
             else w = img[kv_v_at(t, d)] | img[kv_v_at(t, d + 1u)] << 8 | img[kv_v_at(t, d + 2u)] << 16 | img[kv_v_at(t, d + 3u)] << 24;
 #pragma unroll
-            for (uint32_t e = 0; e < 4u; ++e) v[e] = s * static_cast<float>(static_cast<int>((w >> (8u * e)) & 255u) - 128);
+            for (uint32_t e = 0; e < 4u; ++e) v[e] = s * (static_cast<float>((w >> (8u * e)) & 255u) - 128.0f);
         } else {
             v = *reinterpret_cast<const f4*>(old + t * c.hdp + d);
         }
@@ -296,27 +305,31 @@ __device__ __forceinline__ KvSpan kv_span(const Kv8AttnArgs& A, const Kv8Seq& S,
     return r;
 }
 
-// Four biased codes to f16: the byte under 0x64 is 1024 + u, exactly.
-__device__ __forceinline__ void kv_cvt4(uint32_t w, h2& a, h2& b) {
+// Biased bytes to halves: the byte under 0x64 is 1024 + q + 128, exactly, and 1152 comes off. (As the half's low bits alone, (q + 128)
+// 2^-24, a key takes no subtraction, but 128 times the sum of the queries has to come off the scores: five times the error.
+// Signs and magnitudes kept so that they are subnormals right away lose digits: the matrix cores drop the product of two
+// subnormals, and the low parts of small weights are such, 1.7e-4 of the outputs at 8192 positions.)
+__device__ __forceinline__ h8 kv_halves(uint32_t w0, uint32_t w1) {
     const h2 off = {static_cast<_Float16>(-1152.0f), static_cast<_Float16>(-1152.0f)};
-    a = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)) + off;
-    b = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)) + off;
-}
-__device__ __forceinline__ h8 kv_cvt8(uint32_t w0, uint32_t w1) {
-    h2 a, b, c, d;
-    kv_cvt4(w0, a, b);
-    kv_cvt4(w1, c, d);
+    const h2 a = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w0, 0x04010400u)) + off;
+    const h2 b = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w0, 0x04030402u)) + off;
+    const h2 c = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w1, 0x04010400u)) + off;
+    const h2 d = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w1, 0x04030402u)) + off;
     return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// tanh(x): below 1/4 its series (the next term is 9e-9 of it), above by e^(-2|x|), at 1 ulp each of exponential and
-// reciprocal.
-__device__ __forceinline__ float kv_tanh(float x) {
-    const float a = fabsf(x), y = x * x;
-    const float e = __builtin_amdgcn_exp2f(a * -2.885390082f);
-    const float big = (1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e);
-    const float small = x + x * y * (-0.3333333333f + y * (0.1333333333f + y * (-0.05396825397f + y * 0.02186948854f)));
-    return a < 0.25f ? small : copysignf(big, x);
+// tanh(x). Up to 1/2 in magnitude its odd polynomial of degree 11 (a least-squares fit, relative error 4e-10); above, by
+// e^(-2|x|), at 1 ulp each of exponential and reciprocal. `some`: whether a lane is above, wave-uniform, so that the scores of most
+// blocks, well below the cap, cost no exponential here.
+__device__ __forceinline__ float kv_tanh(float x, bool some) {
+    const float y = x * x;
+    float r = x + x * y * (-0.33333327f + y * (0.13332961f + y * (-0.05389886f + y * (0.02129668f + y * -0.0066456f))));
+    if (some) {
+        const float a = fabsf(x), e = __builtin_amdgcn_exp2f(a * -2.885390082f);
+        const float big = (1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e);
+        r = a <= 0.5f ? r : copysignf(big, x);
+    }
+    return r;
 }
 
 #define KV_MFMA(a, b, c) __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0)
@@ -330,56 +343,82 @@ __device__ __forceinline__ float max_xor32(float v) {
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-// What a wave holds of RT tiles of 16 query rows (lane l: row l % 16 of each). The queries are the B operand of the transposed
-// scores (lane l: dims 32 s + 8 (l / 16) + e), scaled by a power of two to below 2^14 and split into halves. The outputs are
-// transposed too (dims 16 t + 4 (l / 16) + e), in units of 2^(eR - 9).
+// Pairs of floats to pairs of halves, hi + lo = x. (The barrier: see gm_split.)
+__device__ __forceinline__ void kv_split2(float x, float y, h2& hi, h2& lo) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    asm("" : "+v"(x), "+v"(y));
+    hi = __builtin_convertvector((f2{x, y}), h2);
+    lo = __builtin_convertvector((f2{x - static_cast<float>(hi[0]), y - static_cast<float>(hi[1])}), h2);
+}
+
+// Queries are the B operand of the transposed scores (lane l: row l % 16, dims 32 s + 8 (l / 16) + e), each row scaled by a power
+// of two to below 2^14 and split into halves: units (s, high or low) of 64 lanes x 16 bytes. One tile of 16 rows stays in
+// registers; of more, which all waves of a workgroup share, they stay in LDS, so that the outputs' registers leave
+// room for two waves a SIMD.
+template <int NT>
+struct KvQuery {
+    h8 q[NT][2];
+};
+// Rows r0 .. r0 + 15; f: a score's factor but for its key's scale (log2 units without a cap).
+template <int NT, bool CAP>
+__device__ __forceinline__ void kv_load_q(const Kv8AttnArgs& A, const Kv8Seq& S, uint32_t kvh, uint32_t r0, KvQuery<NT>& Q, float& f) {
+    const uint32_t lane = threadIdx.x & 63u, R = S.n * A.G, hd = A.c.hd;
+    const uint32_t r = min(r0 + (lane & 15u), R - 1u), qi = r / A.G, h = kvh * A.G + (r - qi * A.G);
+    const float* src = A.q + (static_cast<uint64_t>(S.row0) + qi) * A.q_stride + h * hd;
+    f4 x[NT][2];
+    float m = 0.0f;
+#pragma unroll
+    for (int s = 0; s < NT; ++s)
+#pragma unroll
+        for (uint32_t j = 0; j < 2u; ++j) {
+            const uint32_t d = 32u * s + 8u * (lane >> 4) + 4u * j;
+            x[s][j] = *reinterpret_cast<const f4*>(src + min(d, hd - 4u));
+            if (d >= hd) x[s][j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+#pragma unroll
+    for (int s = 0; s < NT; ++s)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(x[s][j >> 2][j & 3]));
+    m = max_xor32(max_xor16(m));
+    const int ex = kv_exp(m, 14);
+    const float sign = A.scale < 0.0f ? -1.0f : 1.0f;   // factors are not negative: the largest score is the largest product
+    f = ldexpf(1.0f, -ex) * (fabsf(A.scale) * (CAP ? 1.0f : 1.4426950409f));
+    const float up = ldexpf(sign, ex);
+#pragma unroll
+    for (int s = 0; s < NT; ++s)
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+            h2 a, b;
+            kv_split2(x[s][j >> 2][j & 3] * up, x[s][j >> 2][(j & 3) + 1] * up, a, b);
+            Q.q[s][0][j] = a[0], Q.q[s][0][j + 1] = a[1];
+            Q.q[s][1][j] = b[0], Q.q[s][1][j + 1] = b[1];
+        }
+}
+
+// What a wave holds of RT tiles of 16 rows (lane l: row l % 16 of each). The outputs are transposed too (dims 16 t + 4 (l / 16) + e), in
+// units of 2^(eR - 9).
 constexpr float kKvGrow = 6.0f;   // weights may pass 1 by 2^6 before the reference maximum follows
 template <int NT, int RT>
 struct KvWave {
-    h8 qh[RT][NT], ql[RT][NT];
+    KvQuery<NT> q;    // RT == 1; else
+    const h8* sq;     //   in LDS: [RT][NT][2][64], from this lane's place on
     f4 acc[RT][2 * NT];
-    float f[RT];      // a score's factor but for its key's scale
+    float f[RT];
     uint32_t p[RT];   // the rows' positions
     float m[RT], l[RT];
     int eR;           // 2^eR is above every value scale so far
+    __device__ __forceinline__ h8 query(int k, int s, int part) const {
+        if constexpr (RT == 1) return q.q[s][part];
+        else return sq[((k * NT + s) * 2 + part) * 64];
+    }
 };
-
-template <int NT, int RT, bool CAP>
-__device__ __forceinline__ void kv_start(const Kv8AttnArgs& A, const Kv8Seq& S, uint32_t kvh, uint32_t r0, KvWave<NT, RT>& W) {
-    const uint32_t lane = threadIdx.x & 63u, R = S.n * A.G, hd = A.c.hd;
+template <int NT, int RT>
+__device__ __forceinline__ void kv_start(const Kv8AttnArgs& A, const Kv8Seq& S, uint32_t r0, KvWave<NT, RT>& W) {
 #pragma unroll
     for (int k = 0; k < RT; ++k) {
-        const uint32_t r = min(r0 + 16u * k + (lane & 15u), R - 1u), qi = r / A.G, h = kvh * A.G + (r - qi * A.G);
-        const float* src = A.q + (static_cast<uint64_t>(S.row0) + qi) * A.q_stride + h * hd;
-        f4 x[NT][2];
-        float m = 0.0f;
-#pragma unroll
-        for (int s = 0; s < NT; ++s)
-#pragma unroll
-            for (uint32_t j = 0; j < 2u; ++j) {
-                const uint32_t d = 32u * s + 8u * (lane >> 4) + 4u * j;
-                x[s][j] = d < hd ? *reinterpret_cast<const f4*>(src + d) : f4{0.0f, 0.0f, 0.0f, 0.0f};
-            }
-#pragma unroll
-        for (int s = 0; s < NT; ++s)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(x[s][j >> 2][j & 3]));
-        m = max_xor32(max_xor16(m));
-        const int ex = kv_exp(m, 14);
-        const float sign = A.scale < 0.0f ? -1.0f : 1.0f;   // factors are not negative: the largest score is the largest product
-        W.f[k] = ldexpf(1.0f, -ex) * (fabsf(A.scale) * (CAP ? 1.0f : 1.4426950409f));
-        W.p[k] = S.pos + qi;
+        W.p[k] = S.pos + min(r0 + 16u * k + (threadIdx.x & 15u), S.n * A.G - 1u) / A.G;
         W.m[k] = -INFINITY;
         W.l[k] = 0.0f;
-#pragma unroll
-        for (int s = 0; s < NT; ++s)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                _Float16 a, b;
-                kv_split(ldexpf(x[s][j >> 2][j & 3] * sign, ex), a, b);
-                W.qh[k][s][j] = a;
-                W.ql[k][s][j] = b;
-            }
 #pragma unroll
         for (int t = 0; t < 2 * NT; ++t) W.acc[k][t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
     }
@@ -405,17 +444,15 @@ __device__ __forceinline__ void kv_scores(const KvRaw<NT>& K, const KvWave<NT, R
     for (int k = 0; k < RT; ++k) s[k][0] = s[k][1] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        const h8 a0 = kv_cvt8(K.w[t].x, K.w[t].y), a1 = kv_cvt8(K.w[t].z, K.w[t].w);
+        const h8 a0 = kv_halves(K.w[t].x, K.w[t].y), a1 = kv_halves(K.w[t].z, K.w[t].w);
 #pragma unroll
-        for (int k = 0; k < RT; ++k) {
-            s[k][0] = KV_MFMA(a0, W.qh[k][t], s[k][0]);
-            s[k][1] = KV_MFMA(a1, W.qh[k][t], s[k][1]);
-        }
+        for (int part = 0; part < 2; ++part)
 #pragma unroll
-        for (int k = 0; k < RT; ++k) {
-            s[k][0] = KV_MFMA(a0, W.ql[k][t], s[k][0]);
-            s[k][1] = KV_MFMA(a1, W.ql[k][t], s[k][1]);
-        }
+            for (int k = 0; k < RT; ++k) {
+                const h8 q = W.query(k, t, part);
+                s[k][0] = KV_MFMA(a0, q, s[k][0]);
+                s[k][1] = KV_MFMA(a1, q, s[k][1]);
+            }
     }
 }
 // The same of the open block, from the tail's pairs.
@@ -432,9 +469,10 @@ __device__ __forceinline__ void kv_scores_open(const Kv8Dev& c, uint64_t buf, co
             const h8 a = hi[64 * (2 * t + half)], b = lo[64 * (2 * t + half)];
 #pragma unroll
             for (int k = 0; k < RT; ++k) {
-                s[k][half] = KV_MFMA(a, W.qh[k][t], s[k][half]);
-                s[k][half] = KV_MFMA(a, W.ql[k][t], s[k][half]);
-                s[k][half] = KV_MFMA(b, W.qh[k][t], s[k][half]);
+                const h8 q = W.query(k, t, 0);
+                s[k][half] = KV_MFMA(a, q, s[k][half]);
+                s[k][half] = KV_MFMA(b, q, s[k][half]);
+                s[k][half] = KV_MFMA(a, W.query(k, t, 1), s[k][half]);
             }
         }
 }
@@ -442,13 +480,16 @@ __device__ __forceinline__ void kv_scores_open(const Kv8Dev& c, uint64_t buf, co
 // Tokens of a lane's eight scores.
 __device__ __forceinline__ uint32_t kv_token(uint32_t e) { return 4u * ((threadIdx.x & 63u) >> 4) + (e & 3u) + 16u * (e >> 2); }
 
-// One block's scores to weights: x in log2 units, running reference maximum and sum, the weights times the values'
-// scale as pairs of halves. ks / vs: the block's scales, or (OPEN) those of the lane's tokens. dump: where the row's scores go.
+// One block's scores to weights: log2 units, running reference maximum and sum, the weights times the values' scale as
+// pairs of halves. ks / vs: the block's scales, or (OPEN) those of the lane's tokens. dump: where
+// the row's scores go.
 template <int NT, int RT, bool CAP, bool OPEN>
-__device__ __forceinline__ void kv_soft(const Kv8AttnArgs& A, const Kv8Seq& S, uint32_t b, bool masked, const f4 (&s)[RT][2],
+__device__ __forceinline__ void kv_soft(const Kv8AttnArgs& A, const Kv8Seq& S, uint32_t b, bool masked, f4 (&s)[RT][2],
                                         const float* ks, const float* vs, KvWave<NT, RT>& W, h8 (&ph)[RT], h8 (&pl)[RT], float* dump) {
-    float x[RT][8], top[RT];
-    uint32_t see[RT];   // bit e
+    float F[RT], top[RT];   // a score in log2 units is s F (but for a cap or an open block: s is that already)
+    uint32_t see[RT];              // bit e
+    const bool direct = CAP || OPEN;
+    bool some = false;
 #pragma unroll
     for (int k = 0; k < RT; ++k) {
         see[k] = 0xffu;
@@ -462,15 +503,27 @@ __device__ __forceinline__ void kv_soft(const Kv8AttnArgs& A, const Kv8Seq& S, u
                 see[k] |= static_cast<uint32_t>(y) << e;
             }
         }
-        top[k] = -INFINITY;
+        F[k] = OPEN ? W.f[k] : W.f[k] * ks[0];
+        if constexpr (direct) {
+            const float rc = CAP ? 1.0f / A.cap : 1.0f;
 #pragma unroll
-        for (uint32_t e = 0; e < 8u; ++e) {
-            x[k][e] = s[k][e >> 2][e & 3u] * (W.f[k] * (OPEN ? ks[e] : ks[0]));
-            if constexpr (CAP) x[k][e] = A.cap * 1.4426950409f * kv_tanh(x[k][e] * (1.0f / A.cap));
-            if (masked) x[k][e] = (see[k] >> e) & 1u ? x[k][e] : -INFINITY;
-            top[k] = fmaxf(top[k], x[k][e]);
+            for (uint32_t e = 0; e < 8u; ++e) {
+                float x = s[k][e >> 2][e & 3u];
+                x *= OPEN ? F[k] * ks[e] : F[k];
+                if constexpr (CAP) {
+                    x *= rc;
+                    some |= fabsf(x) > 0.5f;
+                }
+                s[k][e >> 2][e & 3u] = x;
+            }
         }
-        top[k] = max_xor32(max_xor16(top[k]));
+    }
+    if constexpr (CAP) {
+        some = __any(some);
+#pragma unroll
+        for (int k = 0; k < RT; ++k)
+#pragma unroll
+            for (uint32_t e = 0; e < 8u; ++e) s[k][e >> 2][e & 3u] = A.cap * 1.4426950409f * kv_tanh(s[k][e >> 2][e & 3u], some);
     }
     float v = OPEN ? 0.0f : vs[0];
     if constexpr (OPEN) {
@@ -481,7 +534,17 @@ __device__ __forceinline__ void kv_soft(const Kv8AttnArgs& A, const Kv8Seq& S, u
     const int ev = v > 0.0f && v < INFINITY ? __builtin_amdgcn_frexp_expf(v) : kKvNoExp;
     bool grow = ev > W.eR;
 #pragma unroll
-    for (int k = 0; k < RT; ++k) grow |= top[k] > W.m[k] + kKvGrow;
+    for (int k = 0; k < RT; ++k) {
+        if (masked)
+#pragma unroll
+            for (uint32_t e = 0; e < 8u; ++e) s[k][e >> 2][e & 3u] = (see[k] >> e) & 1u ? s[k][e >> 2][e & 3u] : -INFINITY;
+        float t = -INFINITY;
+#pragma unroll
+        for (uint32_t e = 0; e < 8u; ++e) t = fmaxf(t, s[k][e >> 2][e & 3u]);
+        t = max_xor32(max_xor16(t));
+        top[k] = direct || t == -INFINITY ? t : t * F[k];
+        grow |= top[k] > W.m[k] + kKvGrow;
+    }
     if (__any(grow)) {
         const int eR = max(W.eR, ev);
 #pragma unroll
@@ -499,28 +562,37 @@ __device__ __forceinline__ void kv_soft(const Kv8AttnArgs& A, const Kv8Seq& S, u
         W.eR = eR;
     }
     const int up = W.eR == kKvNoExp ? 0 : 9 - W.eR;
+    const float vf = OPEN ? 0.0f : ldexpf(vs[0], up);
 #pragma unroll
     for (int k = 0; k < RT; ++k) {
         const float ref = W.m[k] == -INFINITY ? 0.0f : W.m[k];
         float p[8];
 #pragma unroll
         for (uint32_t e = 0; e < 8u; ++e) {
-            p[e] = __builtin_amdgcn_exp2f(x[k][e] - ref);
+            const float x = s[k][e >> 2][e & 3u];
+            p[e] = __builtin_amdgcn_exp2f(direct ? x - ref : __builtin_fmaf(x, F[k], -ref));
+            if (masked) p[e] = (see[k] >> e) & 1u ? p[e] : 0.0f;
             W.l[k] += p[e];
-            p[e] *= ldexpf(OPEN ? vs[e] : vs[0], up);
+            p[e] *= OPEN ? ldexpf(vs[e], up) : vf;
             if (masked) p[e] = (see[k] >> e) & 1u ? p[e] : 0.0f;   // (0 times a scale that is NaN)
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            _Float16 a, d;
-            kv_split(p[e], a, d);
-            ph[k][e] = a;
-            pl[k][e] = d;
+        for (int e = 0; e < 8; e += 2) {
+            h2 a, d;
+            kv_split2(p[e], p[e + 1], a, d);
+            ph[k][e] = a[0], ph[k][e + 1] = a[1];
+            pl[k][e] = d[0], pl[k][e + 1] = d[1];
         }
     }
     if (dump) {
-        *reinterpret_cast<f4*>(dump) = f4{x[0][0], x[0][1], x[0][2], x[0][3]};
-        *reinterpret_cast<f4*>(dump + 16) = f4{x[0][4], x[0][5], x[0][6], x[0][7]};
+        f4 x[2];
+#pragma unroll
+        for (uint32_t e = 0; e < 8u; ++e) {
+            const float y = s[0][e >> 2][e & 3u];
+            x[e >> 2][e & 3u] = direct || y == -INFINITY ? y : y * F[0];
+        }
+        *reinterpret_cast<f4*>(dump) = x[0];
+        *reinterpret_cast<f4*>(dump + 16) = x[1];
     }
 }
 
@@ -528,7 +600,7 @@ template <int NT, int RT>
 __device__ __forceinline__ void kv_values(const KvRaw<NT>& V, const h8 (&ph)[RT], const h8 (&pl)[RT], KvWave<NT, RT>& W) {
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        const h8 a0 = kv_cvt8(V.w[t].x, V.w[t].y), a1 = kv_cvt8(V.w[t].z, V.w[t].w);
+        const h8 a0 = kv_halves(V.w[t].x, V.w[t].y), a1 = kv_halves(V.w[t].z, V.w[t].w);
 #pragma unroll
         for (int k = 0; k < RT; ++k) {
             W.acc[k][2 * t] = KV_MFMA(a0, ph[k], W.acc[k][2 * t]);
@@ -609,90 +681,127 @@ __device__ __forceinline__ void kv_row_done(const Kv8AttnArgs& A, uint32_t row, 
     if (A.o.nonfinite && (!(L > 0.0f) || !__builtin_isfinite(L))) atomicMin(A.o.nonfinite, A.o.code);
 }
 
-// The virtual blocks i0, i0 + step, ... below i1 of a wave's rows (span sp). The keys of the next block are loaded while
-// this one's weights are computed, its values while the next scores are.
-template <int NT, int RT, bool CAP>
+// The virtual blocks i0, i0 + 4, ... below i1 of a wave's rows (span sp). The keys of the next block are loaded while
+// this one's weights are computed, its values while the next scores are; the first block's before start() makes the queries.
+template <int NT, int RT, bool CAP, class Start>
 __device__ __forceinline__ void kv_run(const Kv8AttnArgs& A, const Kv8Seq& S, uint32_t kvh, const KvSpan& sp, uint32_t pmin, uint32_t pmax,
-                                       uint32_t i0, uint32_t i1, uint32_t step, KvWave<NT, RT>& W, float* dump) {
+                                       uint32_t i0, uint32_t i1, KvWave<NT, RT>& W, float* dump, Start start) {
     const Kv8Dev& c = A.c;
     auto block = [&](uint32_t i) { return i < sp.n_pre ? i : sp.lo + (i - sp.n_pre); };
     const uint32_t last = block(sp.n - 1u);
     const bool open = (last + 1u) * 32u > S.pos + S.n;   // the last virtual block
     const uint32_t e1 = open ? min(i1, sp.n - 1u) : i1;
+    KvRaw<NT> K, V;
+    float2 sc = {0.0f, 0.0f};
+    const bool any = i0 < e1;
+    // (a wave without a full block loads one all the same, the first of the region, and uses nothing of it)
+    uint64_t blk = kv_block(c, S.seq, kvh, any ? block(i0) : 0u);
+    kv_load<NT>(c, blk, 0u, K);
+    kv_load<NT>(c, blk, 1u, V);
+    sc = c.scales[blk];
+    __builtin_amdgcn_sched_barrier(0);
+    start();
     uint32_t i = i0;
-    if (i < e1) {
-        KvRaw<NT> K, V;
-        uint64_t blk = kv_block(c, S.seq, kvh, block(i));
+    for (; i < e1; i += 4u) {
+        const uint32_t b = block(i);
+        f4 s[RT][2];
+        kv_scores<NT, RT>(K, W, s);
+        // (the last block's "next" is itself, again in cache: with no branch, a wait counts the loads it is for alone)
+        blk = kv_block(c, S.seq, kvh, block(i + 4u < e1 ? i + 4u : i));
         kv_load<NT>(c, blk, 0u, K);
+        const float2 cur = sc;
+        sc = c.scales[blk];
+        __builtin_amdgcn_sched_barrier(0);   // the loads are issued here, and not next to their use
+        h8 ph[RT], pl[RT];
+        kv_soft<NT, RT, CAP, false>(A, S, b, kv_masked(A, S, b, pmin, pmax), s, &cur.x, &cur.y, W, ph, pl,
+                                    dump ? dump + 32u * (i - i0) : nullptr);
+        kv_values<NT, RT>(V, ph, pl, W);
         kv_load<NT>(c, blk, 1u, V);
-        float2 sc = c.scales[blk];
-        for (; i < e1; i += step) {
-            const uint32_t b = block(i);
-            f4 s[RT][2];
-            kv_scores<NT, RT>(K, W, s);
-            const bool more = i + step < e1;
-            const float2 cur = sc;
-            if (more) {
-                blk = kv_block(c, S.seq, kvh, block(i + step));
-                kv_load<NT>(c, blk, 0u, K);
-                sc = c.scales[blk];
-            }
-            h8 ph[RT], pl[RT];
-            kv_soft<NT, RT, CAP, false>(A, S, b, kv_masked(A, S, b, pmin, pmax), s, &cur.x, &cur.y, W, ph, pl,
-                                        dump ? dump + 32u * (i - i0) : nullptr);
-            kv_values<NT, RT>(V, ph, pl, W);
-            if (more) kv_load<NT>(c, blk, 1u, V);
-        }
+        __builtin_amdgcn_sched_barrier(0);
     }
     if (open && i == sp.n - 1u && i < i1) kv_open<NT, RT, CAP>(A, S, kvh, last, W, dump ? dump + 32u * (i - i0) : nullptr);
 }
 
-// Single tokens, and a few: one workgroup per (split of a 16-row unit's blocks, head, sequence), its waves taking every fourth
-// block and meeting in LDS, eight rows at a time.
-template <int NT, bool CAP>
+// One workgroup per (split of a unit's blocks, head, sequence), its waves taking every fourth block and meeting in LDS, eight rows
+// at a time. A unit is 16 RT rows: 16 for single tokens (memory's time: two workgroups a CU hold 16 KB a wave in
+// flight); more for prompts, where a block's codes become halves once for all of a wave's rows. A sequence's units come the
+// longest first, so that what is left at the end is short (or, where all run at once, so that a CU's two are as long
+// together as any other's); the (head, sequence)s side by side: eight of them or a multiple have an XCD's L2 each.
+template <int NT, int RT, bool CAP>
 __global__ void __launch_bounds__(kKvThreads, 2) k_kv8_attn(const Kv8AttnArgs A) {
     constexpr uint32_t HDP = 32u * NT, C4 = HDP / 4u;
-    __shared__ __align__(16) f4 s_acc[4][8 * C4];
-    __shared__ float s_m[4][16], s_l[4][16];
-    const Kv8Seq& S = A.s[blockIdx.z];
-    const uint32_t kvh = blockIdx.y, unit = blockIdx.x / A.splits, split = blockIdx.x - unit * A.splits;
-    const uint32_t R = S.n * A.G, r0 = 16u * unit;
-    if (r0 >= R || split >= S.splits) return;
+    constexpr uint32_t kMeet = 4u * 8u * C4, kQ = RT > 1 ? RT * NT * 128u : 0u;   // units of 16 bytes: the waves' outputs; queries
+    __shared__ __align__(16) f4 s_buf[kMeet > kQ ? kMeet : kQ];
+    __shared__ float s_m[4][16 * RT], s_l[4][16 * RT], s_f[16 * RT];
+    f4* const s_acc = s_buf;   // [4][8 C4], after the queries' last use
+    const uint32_t pairs = A.nseq * A.c.kvh, pair = blockIdx.x % pairs, rest = blockIdx.x / pairs;
+    const uint32_t kvh = pair % A.c.kvh, split = rest % A.splits;
+    const Kv8Seq& S = A.s[pair / A.c.kvh];
+    const uint32_t R = S.n * A.G, units = (R + 16u * RT - 1u) / (16u * RT), at = rest / A.splits;
+    if (at >= units || split >= S.splits) return;
+    const uint32_t unit = A.fold && at >= units / 2u ? at - units / 2u : units - 1u - at;
+    const uint32_t r0 = 16u * RT * unit, rows = min(16u * RT, R - r0);
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, m16 = lane & 15u;
-    const uint32_t pmin = S.pos + r0 / A.G, pmax = S.pos + min(r0 + 15u, R - 1u) / A.G;
+    const uint32_t pmin = S.pos + r0 / A.G, pmax = S.pos + (r0 + rows - 1u) / A.G;
     const KvSpan sp = kv_span(A, S, pmin, pmax);
-    const uint32_t i0 = split * A.per, i1 = min(sp.n, i0 + A.per), rows = min(16u, R - r0);
+    const uint32_t i0 = split * A.per, i1 = min(sp.n, i0 + A.per);
     if (i0 >= i1) return;
     const uint64_t place = static_cast<uint64_t>(S.part0) + (unit * A.c.kvh + kvh) * S.splits + split;
     float* dump = nullptr;   // this lane's row of the unit's scores
-    if (A.scores && m16 < rows) dump = A.scores + (place * A.lines + m16) * 32u * A.per + 32u * wave + 4u * g;
-    KvWave<NT, 1> W;
-    kv_start<NT, 1, CAP>(A, S, kvh, r0, W);
-    kv_run<NT, 1, CAP>(A, S, kvh, sp, pmin, pmax, i0 + wave, i1, 4u, W, dump);
-    float l = add_xor32(add_xor16(W.l[0]));
-    if (g == 0u) {
-        s_m[wave][m16] = W.m[0];
-        s_l[wave][m16] = l;
+    if (RT == 1 && A.scores && m16 < rows) dump = A.scores + (place * A.lines + m16) * 32u * A.per + 32u * wave + 4u * g;
+    KvWave<NT, RT> W;
+    kv_run<NT, RT, CAP>(A, S, kvh, sp, pmin, pmax, i0 + wave, i1, W, dump, [&]() {
+        if constexpr (RT == 1) {
+            kv_load_q<NT, CAP>(A, S, kvh, r0, W.q, W.f[0]);
+        } else {
+            h8* sq = reinterpret_cast<h8*>(s_buf) + lane;
+            if (wave < RT) {   // a tile each
+                KvQuery<NT> Q;
+                float f;
+                kv_load_q<NT, CAP>(A, S, kvh, r0 + 16u * wave, Q, f);
+#pragma unroll
+                for (int s = 0; s < NT; ++s)
+#pragma unroll
+                    for (int part = 0; part < 2; ++part) sq[((wave * NT + s) * 2u + part) * 64u] = Q.q[s][part];
+                if (g == 0u) s_f[16u * wave + m16] = f;
+            }
+            __syncthreads();
+            W.sq = sq;
+#pragma unroll
+            for (int k = 0; k < RT; ++k) W.f[k] = s_f[16 * k + m16];
+        }
+        kv_start<NT, RT>(A, S, r0, W);
+    });
+#pragma unroll
+    for (int k = 0; k < RT; ++k) {
+        const float l = add_xor32(add_xor16(W.l[k]));
+        if (g == 0u) {
+            s_m[wave][16 * k + m16] = W.m[k];
+            s_l[wave][16 * k + m16] = l;
+        }
     }
     __syncthreads();
-    const float M = fmaxf(fmaxf(s_m[0][m16], s_m[1][m16]), fmaxf(s_m[2][m16], s_m[3][m16]));
-    const float ref = M == -INFINITY ? 0.0f : M;
-    const float mine = __builtin_amdgcn_exp2f(W.m[0] - ref);
     const bool only = S.splits == 1u;
-    for (uint32_t h0 = 0; h0 < rows; h0 += 8u) {
-        if (h0) __syncthreads();
-        if (m16 - h0 < 8u)
+#pragma unroll
+    for (int q = 0; q < 2 * RT; ++q) {   // rows 8 q .. 8 q + 7
+        if (8u * q >= rows) break;
+        if (q) __syncthreads();
+        if (m16 >> 3 == (q & 1u)) {
+            const uint32_t k = q >> 1, row = 16u * k + m16;
+            const float M = fmaxf(fmaxf(s_m[0][row], s_m[1][row]), fmaxf(s_m[2][row], s_m[3][row]));
+            const float mine = __builtin_amdgcn_exp2f(W.m[k] - (M == -INFINITY ? 0.0f : M));
 #pragma unroll
             for (int t = 0; t < 2 * NT; ++t) {
                 f4 v;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = ldexpf(W.acc[0][t][e], W.eR - 9) * mine;
-                s_acc[wave][(m16 - h0) * C4 + ((4u * t + g) ^ (m16 & 7u))] = v;   // (rows spread over the banks)
+                for (int e = 0; e < 4; ++e) v[e] = ldexpf(W.acc[k][t][e], W.eR - 9) * mine;
+                s_acc[(wave * 8u + (m16 & 7u)) * C4 + ((4u * t + g) ^ (m16 & 7u))] = v;   // (rows spread over the banks)
             }
+        }
         __syncthreads();
-        for (uint32_t u = threadIdx.x; u < min(8u, rows - h0) * C4; u += kKvThreads) {
-            const uint32_t rr = u / C4, c4 = u - rr * C4, row = h0 + rr, at = rr * C4 + (c4 ^ (rr & 7u));
-            const f4 v = (s_acc[0][at] + s_acc[1][at]) + (s_acc[2][at] + s_acc[3][at]);
+        for (uint32_t u = threadIdx.x; u < min(8u, rows - 8u * q) * C4; u += kKvThreads) {
+            const uint32_t rr = u / C4, c4 = u - rr * C4, row = 8u * q + rr, at4 = rr * C4 + (c4 ^ rr);
+            const f4 v = (s_acc[at4] + s_acc[8u * C4 + at4]) + (s_acc[16u * C4 + at4] + s_acc[24u * C4 + at4]);
             const float m = fmaxf(fmaxf(s_m[0][row], s_m[1][row]), fmaxf(s_m[2][row], s_m[3][row]));
             const float rf = m == -INFINITY ? 0.0f : m;
             float L = 0.0f;
@@ -700,62 +809,12 @@ __global__ void __launch_bounds__(kKvThreads, 2) k_kv8_attn(const Kv8AttnArgs A)
             for (int w = 0; w < 4; ++w) L += s_l[w][row] * __builtin_amdgcn_exp2f(s_m[w][row] - rf);
             if (only) {
                 const uint32_t r = r0 + row, qi = r / A.G, h = kvh * A.G + (r - qi * A.G);
-                if (4u * c4 < A.c.hd) kv_give(A, S.row0 + qi, h, 4u * c4, v / L);
+                if (4u * c4 < A.c.hd) kv_give(A, S.row0 + qi, h, 4u * c4, v * (1.0f / L));
                 if (c4 == 0u) kv_row_done(A, S.row0 + qi, h, m, L);
             } else {
                 *reinterpret_cast<f4*>(A.part + (place * A.lines + row) * HDP + 4u * c4) = v;
             }
             if (c4 == 0u && (!only || A.scores)) A.part_ml[place * A.lines + row] = make_float2(m, L);
-        }
-    }
-}
-
-// Prompts: a wave per unit of 16 RT rows and split of its blocks; the four waves of a workgroup have neighbouring units of one
-// head and read the same blocks at about the same time. The units of one (head, sequence) are dealt to workgroups that are a
-// multiple of the (head, sequence)s apart, the longest first: with eight of them or a multiple each has an XCD's L2 to itself.
-template <int NT, int RT, bool CAP>
-__global__ void __launch_bounds__(kKvThreads, 2) k_kv8_prompt(const Kv8AttnArgs A) {
-    const uint32_t pairs = A.nseq * A.c.kvh, pair = blockIdx.x % pairs, rest = blockIdx.x / pairs;
-    const uint32_t kvh = pair % A.c.kvh, split = rest % A.splits;
-    const Kv8Seq& S = A.s[pair / A.c.kvh];
-    const uint32_t R = S.n * A.G, U = 16u * RT, units = (R + U - 1u) / U, group = rest / A.splits;
-    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, m16 = lane & 15u;
-    if (4u * group + wave >= units || split >= S.splits) return;   // whole waves: no barrier follows
-    const uint32_t unit = units - 1u - (4u * group + wave), r0 = U * unit;
-    const uint32_t pmin = S.pos + r0 / A.G, pmax = S.pos + min(r0 + U - 1u, R - 1u) / A.G;
-    const KvSpan sp = kv_span(A, S, pmin, pmax);
-    const uint32_t i0 = split * A.per, i1 = min(sp.n, i0 + A.per);
-    if (i0 >= i1) return;
-    KvWave<NT, RT> W;
-    kv_start<NT, RT, CAP>(A, S, kvh, r0, W);
-    kv_run<NT, RT, CAP>(A, S, kvh, sp, pmin, pmax, i0, i1, 1u, W, nullptr);
-    const bool only = sp.n <= A.per;
-    const uint64_t place = static_cast<uint64_t>(S.part0) + (unit * A.c.kvh + kvh) * S.splits + split;
-#pragma unroll
-    for (int k = 0; k < RT; ++k) {
-        const uint32_t rr = 16u * k + m16, r = r0 + rr;
-        const float L = add_xor32(add_xor16(W.l[k]));
-        if (r >= R) continue;
-        if (only) {
-            const uint32_t qi = r / A.G, h = kvh * A.G + (r - qi * A.G);
-            const float inv = 1.0f / L;
-#pragma unroll
-            for (int t = 0; t < 2 * NT; ++t) {
-                f4 v;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = ldexpf(W.acc[k][t][e], W.eR - 9) * inv;
-                if (16u * t + 4u * g < A.c.hd) kv_give(A, S.row0 + qi, h, 16u * t + 4u * g, v);
-            }
-            if (g == 0u) kv_row_done(A, S.row0 + qi, h, W.m[k], L);
-        } else {
-#pragma unroll
-            for (int t = 0; t < 2 * NT; ++t) {
-                f4 v;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = ldexpf(W.acc[k][t][e], W.eR - 9);
-                *reinterpret_cast<f4*>(A.part + (place * A.lines + rr) * 32u * NT + 16u * t + 4u * g) = v;
-            }
-            if (g == 0u) A.part_ml[place * A.lines + rr] = make_float2(W.m[k], L);
         }
     }
 }
@@ -775,7 +834,7 @@ __global__ void __launch_bounds__(kKvThreads) k_kv8_join(const Kv8AttnArgs A) {
         if (r >= R) return;
         const KvSpan sp = kv_span(A, S, S.pos + unit * U / A.G, S.pos + min(unit * U + U - 1u, R - 1u) / A.G);
         const uint32_t n = (sp.n + A.per - 1u) / A.per;
-        if (S.splits == 1u || (n <= 1u && A.prompt)) return;   // written by the only split
+        if (S.splits == 1u) return;   // written by the only split
         const uint64_t p0 = static_cast<uint64_t>(S.part0) + (unit * c.kvh + kvh) * S.splits;
         float M = -INFINITY;
         for (uint32_t k = lane; k < n; k += 64u) M = fmaxf(M, A.part_ml[(p0 + k) * A.lines + rr].x);
@@ -871,21 +930,39 @@ __global__ void __launch_bounds__(kKvThreads, 2) k_kv8_weights(const Kv8AttnArgs
         if (!in_pre && 32u * b > pmax) continue;
         if (!in_pre && A.window && pmin >= A.window && 32u * b + 31u <= pmin - A.window) break;   // and no later row sees it
         KvWave<NT, 1> W;
-        kv_start<NT, 1, CAP>(A, S, kvh, r0, W);
+        kv_load_q<NT, CAP>(A, S, kvh, r0, W.q, W.f[0]);
         f4 s[1][2];
         if (open) kv_scores_open<NT, 1>(c, kb, W, s);
         else kv_scores<NT, 1>(K, W, s);
         const uint32_t r = r0 + m16;
-        if (r >= R) continue;
-        const uint32_t qi = r / A.G, h = kvh * A.G + (r - qi * A.G);
+        const bool masked = open || r0 + 15u >= R || kv_masked(A, S, b, pmin, pmax);
+        const uint32_t qi = min(r, R - 1u) / A.G, h = kvh * A.G + (min(r, R - 1u) - qi * A.G);
         const float2 st = A.stats[(static_cast<uint64_t>(S.row0) + qi) * A.heads + h];
+        const uint32_t p0 = S.pos + qi;
+        float x[8];
+        bool some = false;
 #pragma unroll
         for (uint32_t e = 0; e < 8u; ++e) {
-            float x = s[0][e >> 2][e & 3u] * (W.f[0] * ks[e]);
-            if constexpr (CAP) x = A.cap * 1.4426950409f * kv_tanh(x * (1.0f / A.cap));
-            const uint32_t j = 32u * b + kv_token(e);
-            const bool y = j < len && (j < S.prefix || (j <= W.p[0] && (!A.window || W.p[0] - j < A.window)));
-            w[e] += y ? __builtin_amdgcn_exp2f(x - st.x) * st.y : 0.0f;
+            x[e] = s[0][e >> 2][e & 3u] * (W.f[0] * ks[e]);
+            if constexpr (CAP) {
+                x[e] *= 1.0f / A.cap;
+                some |= fabsf(x[e]) > 0.5f;
+            }
+        }
+        if constexpr (CAP) {
+            some = __any(some);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = A.cap * 1.4426950409f * kv_tanh(x[e], some);
+        }
+#pragma unroll
+        for (uint32_t e = 0; e < 8u; ++e) {
+            float p = __builtin_amdgcn_exp2f(x[e] - st.x) * st.y;
+            if (masked) {
+                const uint32_t j = 32u * b + kv_token(e);
+                const bool y = r < R && j < len && (j < S.prefix || (j <= p0 && (!A.window || p0 - j < A.window)));
+                p = y ? p : 0.0f;
+            }
+            w[e] += p;
         }
     }
 #pragma unroll
@@ -919,109 +996,180 @@ __device__ __forceinline__ uint32_t kv_key(float w) {
     return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-constexpr uint32_t kKvSelThreads = 1024;
+constexpr uint32_t kKvSelThreads = 1024, kKvSelWaves = kKvSelThreads / 64u, kKvBins = 2048;
 
-// One workgroup per (head, move): the key of the last weight that stays, by four passes of 8 bits, then the positions in
-// order, of those with that key the first ones.
+// One workgroup per (head, move). The key of the last weight that stays, by histograms of its upper 11, middle 11 and lower 10
+// bits; then every wave counts what stays of its run of positions, and writes it, of those with that key the first ones.
 __global__ void __launch_bounds__(kKvSelThreads) k_kv8_select(const Kv8EvictArgs A) {
-    __shared__ uint32_t hist[256], s_bin, s_left;
-    __shared__ uint32_t wsum[2][kKvSelThreads / 64u];
+    __shared__ uint32_t hist[kKvBins], s_bin, s_left, s_gt[kKvSelWaves], s_eq[kKvSelWaves], s_sum[kKvSelWaves];
     const vrt_kv8_move& V = A.m[blockIdx.y];
     const uint32_t head = blockIdx.x, tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
     const float* src = A.w + (static_cast<uint64_t>(V.src) * A.c.kvh + head) * A.max_ctx;
     float* dst = A.w + (static_cast<uint64_t>(V.dst) * A.c.kvh + head) * A.max_ctx;
     uint32_t* kept = A.kept + (static_cast<uint64_t>(blockIdx.y) * A.c.kvh + head) * A.kept_stride;
     const uint32_t old = V.len - V.recent, want = V.keep - V.recent;
-    uint32_t thr = 0u, need = want;   // keys above thr stay, and `need` of those equal to it
-    if (want) {
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            const uint32_t high = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
-            if (tid < 256u) hist[tid] = 0u;
-            __syncthreads();
-            for (uint32_t i = tid; i < old; i += kKvSelThreads) {
-                const uint32_t k = kv_key(src[i]);
-                if ((k & high) == thr) atomicAdd(&hist[(k >> shift) & 255u], 1u);
-            }
-            __syncthreads();
-            if (tid == 0u) {
-                uint32_t left = need, bin = 255u;
-                while (hist[bin] < left) left -= hist[bin--];
-                s_bin = bin;
-                s_left = left;
-            }
-            __syncthreads();
-            thr |= s_bin << shift;
-            need = s_left;
-            __syncthreads();
-        }
-        uint32_t n_kept = 0u, n_eq = 0u;   // so far
-        for (uint32_t i0 = 0; i0 < old; i0 += kKvSelThreads) {
-            const uint32_t i = i0 + tid;
-            const float w = i < old ? src[i] : 0.0f;
-            const uint32_t k = kv_key(w);
-            const bool gt = i < old && k > thr, eq = i < old && k == thr;
-            const uint64_t below = (1ull << lane) - 1ull, be = __ballot(eq);
-            if (lane == 0u) wsum[0][wave] = __popcll(be);
-            __syncthreads();
-            uint32_t eq_at = n_eq + __popcll(be & below), eq_all = 0u;
-            for (uint32_t v = 0; v < kKvSelThreads / 64u; ++v) {
-                if (v < wave) eq_at += wsum[0][v];
-                eq_all += wsum[0][v];
-            }
-            const bool stay = gt || (eq && eq_at < need);
-            const uint64_t bs = __ballot(stay);
-            if (lane == 0u) wsum[1][wave] = __popcll(bs);
-            __syncthreads();
-            uint32_t at = n_kept + __popcll(bs & below), all = 0u;
-            for (uint32_t v = 0; v < kKvSelThreads / 64u; ++v) {
-                if (v < wave) at += wsum[1][v];
-                all += wsum[1][v];
-            }
-            if (stay) {
-                kept[at] = i;
-                dst[at] = w;
-            }
-            n_kept += all;
-            n_eq += eq_all;
-        }
-    }
     for (uint32_t i = tid; i < V.recent; i += kKvSelThreads) {
         kept[want + i] = old + i;
         dst[want + i] = src[old + i];
     }
+    if (want == 0u) return;
+    uint32_t thr = 0u, need = want;   // keys above thr stay, and `need` of those equal to it
+    constexpr uint32_t kShift[3] = {21u, 10u, 0u}, kBits[3] = {11u, 11u, 10u};
+    constexpr uint32_t kAhead = 8u;   // loads in flight
+#pragma unroll
+    for (int pass = 0; pass < 3; ++pass) {
+        const uint32_t shift = kShift[pass], mask = (1u << kBits[pass]) - 1u, high = pass == 0 ? 0u : 0xffffffffu << (shift + kBits[pass]);
+        for (uint32_t i = tid; i < kKvBins; i += kKvSelThreads) hist[i] = 0u;
+        __syncthreads();
+        for (uint32_t i0 = tid; i0 - lane < old; i0 += kKvSelThreads * kAhead) {
+            float w[kAhead];
+#pragma unroll
+            for (uint32_t k = 0; k < kAhead; ++k) w[k] = src[min(i0 + kKvSelThreads * k, old - 1u)];
+#pragma unroll
+            for (uint32_t k = 0; k < kAhead; ++k) {
+                const uint32_t key = kv_key(w[k]), bin = (key >> shift) & mask;
+                const bool in = i0 + kKvSelThreads * k < old && (key & high) == thr;
+                const uint64_t all = __ballot(in);
+                if (!all) continue;
+                // lanes with the same bin as the first of them (often all) add once
+                const uint32_t first = __builtin_amdgcn_readlane(static_cast<int>(bin), __builtin_ctzll(all));
+                const uint64_t same = __ballot(in && bin == first);
+                if (lane == static_cast<uint32_t>(__builtin_ctzll(same))) atomicAdd(&hist[first], static_cast<uint32_t>(__popcll(same)));
+                if (in && bin != first) atomicAdd(&hist[bin], 1u);
+            }
+        }
+        __syncthreads();
+        // bins from the top: thread t has bins kKvBins - 1 - 2 t and the one below
+        const uint32_t hi = hist[kKvBins - 1u - 2u * tid], lo = hist[kKvBins - 2u - 2u * tid];
+        uint32_t run = hi + lo;   // inclusive sums over the wave's threads
+#pragma unroll
+        for (uint32_t o = 1; o < 64u; o <<= 1) {
+            const uint32_t up = __shfl_up(static_cast<int>(run), o);
+            run += lane >= o ? up : 0u;
+        }
+        if (lane == 63u) s_sum[wave] = run;
+        __syncthreads();
+        for (uint32_t v = 0; v < wave; ++v) run += s_sum[v];
+        const uint32_t before = run - hi - lo;
+        if (before < need && need <= run) {   // one thread: the bin that the last one falls into
+            s_bin = before + hi >= need ? kKvBins - 1u - 2u * tid : kKvBins - 2u - 2u * tid;
+            s_left = before + hi >= need ? need - before : need - before - hi;
+        }
+        __syncthreads();
+        thr |= s_bin << shift;
+        need = s_left;
+    }
+    const uint32_t run = ((old + kKvSelWaves - 1u) / kKvSelWaves + 63u) & ~63u, j0 = min(old, run * wave), j1 = min(old, j0 + run);
+    uint32_t n_gt = 0u, n_eq = 0u;
+    for (uint32_t j = j0; j < j1; j += 64u * kAhead) {
+        float w[kAhead];
+#pragma unroll
+        for (uint32_t k = 0; k < kAhead; ++k) w[k] = src[min(j + 64u * k + lane, j1 - 1u)];
+#pragma unroll
+        for (uint32_t k = 0; k < kAhead; ++k) {
+            const uint32_t key = kv_key(w[k]);
+            const bool in = j + 64u * k + lane < j1;
+            n_gt += __popcll(__ballot(in && key > thr));
+            n_eq += __popcll(__ballot(in && key == thr));
+        }
+    }
+    if (lane == 0u) {
+        s_gt[wave] = n_gt;
+        s_eq[wave] = n_eq;
+    }
+    __syncthreads();
+    uint32_t gt = 0u, eq = 0u;   // before this wave's run
+    for (uint32_t v = 0; v < wave; ++v) {
+        gt += s_gt[v];
+        eq += s_eq[v];
+    }
+    const uint64_t below = (1ull << lane) - 1ull;
+    for (uint32_t j = j0; j < j1; j += 64u * kAhead) {
+        float w[kAhead];
+#pragma unroll
+        for (uint32_t k = 0; k < kAhead; ++k) w[k] = src[min(j + 64u * k + lane, j1 - 1u)];
+#pragma unroll
+        for (uint32_t k = 0; k < kAhead; ++k) {
+            const uint32_t key = kv_key(w[k]), i = j + 64u * k + lane;
+            const uint64_t bg = __ballot(i < j1 && key > thr), be = __ballot(i < j1 && key == thr);
+            const uint32_t my_eq = eq + __popcll(be & below), at = gt + __popcll(bg & below) + min(my_eq, need);
+            if (i < j1 && (key > thr || (key == thr && my_eq < need))) {
+                kept[at] = i;
+                dst[at] = w[k];
+            }
+            gt += __popcll(bg);
+            eq += __popcll(be);
+        }
+    }
 }
 
 // One workgroup per (block of the destination, head and K or V, move): the kept values of the source, into a block as
-// the append makes it, or into the tail.
+// the append makes it, or into the tail. Their codes go through LDS as rows of biased bytes. A key's row is 8-byte pieces of its
+// block, 16 bytes from its neighbours': lanes take the pieces of different tokens. A value's is a byte of every 8: lanes take
+// neighbouring dims, 16 bytes (two dims of eight tokens) a load.
+template <int NT>
 __global__ void __launch_bounds__(kKvThreads) k_kv8_gather(const Kv8EvictArgs A) {
-    __shared__ __align__(16) uint8_t img[32 * 256];
-    __shared__ uint32_t red[4];
+#pragma clang fp contract(off)
+    constexpr uint32_t kRow = 32u * NT + 8u;
+    __shared__ __align__(16) uint8_t img[1024 * NT];
+    __shared__ __align__(16) uint8_t raw[32 * kRow];
+    __shared__ uint32_t red[4], s_p[32];
+    __shared__ float s_s[32];
     const Kv8Dev& c = A.c;
     const vrt_kv8_move& V = A.m[blockIdx.z];
     const uint32_t head = blockIdx.y >> 1, z = blockIdx.y & 1u, b = blockIdx.x, tid = threadIdx.x;
     if (32u * b >= V.keep) return;
     const uint32_t* kept = A.kept + (static_cast<uint64_t>(blockIdx.z) * c.kvh + head) * A.kept_stride;
-    const bool closed = (b + 1u) * 32u <= V.keep, tail = b + 1u >= (V.keep - 1u) >> 5;   // the last block and the one before
-    KvTile T;
-    const uint32_t hd4 = c.hd >> 2, units = 32u * hd4;
+    const uint32_t n = min(32u, V.keep - 32u * b), full = V.len >> 5;   // full blocks of the source
+    if (tid < 32u) {
+        const uint32_t p = kept[32u * b + min(tid, n - 1u)];
+        s_p[tid] = p;
+        s_s[tid] = (p >> 5) < full ? reinterpret_cast<const float*>(c.scales + kv_block(c, V.src, head, p >> 5))[z] : 0.0f;
+    }
+    __syncthreads();
+    if (z == 0u) {
+        for (uint32_t i = tid; i < 128u * NT; i += kKvThreads) {   // (8 dims, token)
+            const uint32_t t = i & 31u, q = i >> 5, p = s_p[t];
+            if ((p >> 5) >= full) continue;
+            const uint8_t* blk = kv_codes(c, kv_block(c, V.src, head, p >> 5));
+            *reinterpret_cast<uint2*>(raw + t * kRow + 8u * q) = *reinterpret_cast<const uint2*>(blk + kv_k_at(p & 31u, 8u * q));
+        }
+    } else {
+        for (uint32_t i = tid; i < 512u * NT; i += kKvThreads) {   // (token, dims 32 jj + m and 16 on)
+            const uint32_t m = i & 15u, jj = (i >> 4) % NT, t = (i >> 4) / NT, p = s_p[t], tok = p & 31u;
+            if ((p >> 5) >= full) continue;
+            const uint8_t* blk = kv_codes(c, kv_block(c, V.src, head, p >> 5)) + 32u * c.hdp;
+            const uint4 u = *reinterpret_cast<const uint4*>(blk + jj * 1024u + (((tok >> 2) & 3u) * 16u + m) * 16u);
+            const bool late = tok >> 4;
+            const uint32_t sh = 8u * (tok & 3u);
+            raw[t * kRow + 32u * jj + m] = static_cast<uint8_t>((late ? u.y : u.x) >> sh);
+            raw[t * kRow + 32u * jj + 16u + m] = static_cast<uint8_t>((late ? u.w : u.z) >> sh);
+        }
+    }
+    __syncthreads();
+    const bool closed = n == 32u, tail = b + 1u >= (V.keep - 1u) >> 5;   // the last block and the one before
     const uint64_t buf = kv_tail_buf(c, V.dst, head, b, z);
+    KvTile<NT> T;
 #pragma unroll
-    for (uint32_t k = 0; k < 8u; ++k) {
-        const uint32_t u = tid + kKvThreads * k;
-        T.v[k] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-        if (u >= units) continue;
+    for (int k = 0; k < NT; ++k) {
         uint32_t t, d;
-        kv_unit(u, hd4, t, d);
-        if (32u * b + t >= V.keep) continue;
-        const uint32_t p = kept[32u * b + t];
+        kv_unit<NT>(k, t, d);
+        T.v[k] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (t >= n || d >= c.hd) continue;
+        const uint32_t p = s_p[t];
+        if ((p >> 5) < full) {
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(raw + t * kRow + d);
 #pragma unroll
-        for (uint32_t e = 0; e < 4u; ++e) T.v[k][e] = kv_value(c, V.src, head, z, p, d + e, V.len);
+            for (uint32_t e = 0; e < 4u; ++e) T.v[k][e] = s_s[t] * (static_cast<float>((w >> (8u * e)) & 255u) - 128.0f);
+        } else {
+            T.v[k] = *reinterpret_cast<const f4*>(c.tail + (kv_tail_buf(c, V.src, head, p >> 5, z) * 32u + (p & 31u)) * c.hdp + d);
+        }
         if (tail) *reinterpret_cast<f4*>(c.tail + (buf * 32u + t) * c.hdp + d) = T.v[k];
     }
-    if (closed) kv_close_block(c, T, kv_block(c, V.dst, head, b), z, img, red);
+    if (closed) kv_close_block<NT>(c, T, kv_block(c, V.dst, head, b), z, img, red);
     if (!tail) return;
     __syncthreads();   // the tail's rows are whole: a wave each for their pairs
-    const uint32_t n = min(32u, V.keep - 32u * b), lane = tid & 63u;
+    const uint32_t lane = tid & 63u;
     for (uint32_t t = tid >> 6; t < n; t += kKvThreads / 64u) {
         f4 v = {0.0f, 0.0f, 0.0f, 0.0f};
         if (4u * lane < c.hd) v = *reinterpret_cast<const f4*>(c.tail + (buf * 32u + t) * c.hdp + 4u * lane);
@@ -1141,26 +1289,32 @@ int attn_plan(const vrt_kv8_cache* c, const vrt_kv8_attn* at, const vrt_kv8_rows
 }
 
 // Tiles of 16 rows that a prompt's wave runs together: as many as leave two waves a SIMD.
-constexpr int rows_of(int nt) { return nt <= 4 ? 2 : 1; }
+constexpr int rows_of(int nt) { return nt <= 4 ? 4 : 2; }
 
+enum Kv8Kernel { kKvAppend, kKvRead, kKvToken, kKvPrompt, kKvWeights, kKvGather };
 template <int NT>
-const void* attn_kernel(bool cap, int which) {   // 0 single tokens, 1 prompts, 2 prompts' weights
+const void* kernel_of(Kv8Kernel k, bool cap) {
     constexpr int RT = rows_of(NT);
-    if (which == 0) return cap ? reinterpret_cast<const void*>(&k_kv8_attn<NT, true>) : reinterpret_cast<const void*>(&k_kv8_attn<NT, false>);
-    if (which == 1)
-        return cap ? reinterpret_cast<const void*>(&k_kv8_prompt<NT, RT, true>) : reinterpret_cast<const void*>(&k_kv8_prompt<NT, RT, false>);
-    return cap ? reinterpret_cast<const void*>(&k_kv8_weights<NT, true>) : reinterpret_cast<const void*>(&k_kv8_weights<NT, false>);
+    switch (k) {
+        case kKvAppend: return reinterpret_cast<const void*>(&k_kv8_append<NT>);
+        case kKvRead: return reinterpret_cast<const void*>(&k_kv8_read<NT>);
+        case kKvGather: return reinterpret_cast<const void*>(&k_kv8_gather<NT>);
+        case kKvToken: return cap ? reinterpret_cast<const void*>(&k_kv8_attn<NT, 1, true>) : reinterpret_cast<const void*>(&k_kv8_attn<NT, 1, false>);
+        case kKvPrompt:
+            return cap ? reinterpret_cast<const void*>(&k_kv8_attn<NT, RT, true>) : reinterpret_cast<const void*>(&k_kv8_attn<NT, RT, false>);
+        default: return cap ? reinterpret_cast<const void*>(&k_kv8_weights<NT, true>) : reinterpret_cast<const void*>(&k_kv8_weights<NT, false>);
+    }
 }
-const void* attn_kernel(uint32_t nt, bool cap, int which) {
-    switch (nt) {
-        case 1: return attn_kernel<1>(cap, which);
-        case 2: return attn_kernel<2>(cap, which);
-        case 3: return attn_kernel<3>(cap, which);
-        case 4: return attn_kernel<4>(cap, which);
-        case 5: return attn_kernel<5>(cap, which);
-        case 6: return attn_kernel<6>(cap, which);
-        case 7: return attn_kernel<7>(cap, which);
-        default: return attn_kernel<8>(cap, which);
+const void* kernel_of(const Kv8Dev& c, Kv8Kernel k, bool cap = false) {
+    switch (c.hdp / 32u) {
+        case 1: return kernel_of<1>(k, cap);
+        case 2: return kernel_of<2>(k, cap);
+        case 3: return kernel_of<3>(k, cap);
+        case 4: return kernel_of<4>(k, cap);
+        case 5: return kernel_of<5>(k, cap);
+        case 6: return kernel_of<6>(k, cap);
+        case 7: return kernel_of<7>(k, cap);
+        default: return kernel_of<8>(k, cap);
     }
 }
 
@@ -1202,8 +1356,9 @@ Kv8Dev kv8_view(const Kv8Sizes& z, void* data, uint32_t kv_heads, uint32_t head_
     return d;
 }
 
-// Single tokens: about 512 workgroups, two a CU, of four blocks at least. Prompts: about 1536 waves' worth of blocks, 16 at least.
-constexpr uint64_t kKvSplits = 512, kKvPromptSplits = 1536;
+// A unit's blocks are split where there are too few units: into about 512 workgroups (two a CU), of four blocks (one a wave) at
+// least. Prompts with as many units as that are not split: their outputs would be written and read once more.
+constexpr uint64_t kKvSplits = 512;
 
 Kv8Plan kv8_plan(Kv8AttnArgs& A, uint32_t kvh, uint32_t hdp, uint32_t n, uint64_t rows, bool scored) {
     Kv8Plan P{};
@@ -1217,15 +1372,17 @@ Kv8Plan kv8_plan(Kv8AttnArgs& A, uint32_t kvh, uint32_t hdp, uint32_t n, uint64_
     A.prompt = rows * A.G > 32ull * active;
     A.unit = A.prompt ? 16u * rows_of(static_cast<int>(hdp / 32u)) : 16u;
     A.lines = std::min(A.unit, std::max(1u, A.rows_most));
-    uint64_t blocks = 0;   // of all units and heads; a prompt's queries see half of its own on average
+    uint64_t units_all = 0, blocks = 0;   // of all units and heads; a prompt's queries see half of its own on average
     for (uint32_t i = 0; i < n; ++i) {
         const Kv8Seq& s = A.s[i];
         const uint32_t most = most_blocks(s, A.window, A.unit);
-        blocks += static_cast<uint64_t>((s.n * A.G + A.unit - 1u) / A.unit) * kvh *
-                  (s.prefix ? most : std::min(most, (s.pos + (s.n + 1u) / 2u + 31u) / 32u));
+        const uint64_t units = static_cast<uint64_t>((s.n * A.G + A.unit - 1u) / A.unit) * kvh;
+        units_all += units;
+        blocks += units * (s.prefix ? most : std::min(most, (s.pos + (s.n + 1u) / 2u + 31u) / 32u));
     }
-    const uint64_t per = A.prompt ? std::max<uint64_t>(16u, (blocks + kKvPromptSplits - 1u) / kKvPromptSplits)
-                                  : std::max<uint64_t>(4u, (blocks + kKvSplits - 1u) / kKvSplits);
+    uint64_t per = std::max<uint64_t>(4u, (blocks + kKvSplits - 1u) / kKvSplits);
+    if (A.prompt && units_all >= kKvSplits / 2u) per = VRT_KV8_MAX_CTX / 32u + 4u;
+    A.fold = A.prompt && units_all <= kKvSplits;
     A.per = static_cast<uint32_t>((per + 3u) & ~3ull);
     A.splits = 1u;
     const bool dump = scored && !A.prompt;
@@ -1267,7 +1424,7 @@ int kv8_append(const Kv8Dev& c, const Kv8Seq* seqs, uint32_t n, const float* k, 
         blocks = std::max(blocks, touched(seqs[i]));
     }
     if (blocks == 0u) return VRT_OK;
-    return launch(reinterpret_cast<const void*>(&k_kv8_append), dim3(blocks, 2u * c.kvh, n), kKvThreads, A, s);
+    return launch(kernel_of(c, kKvAppend), dim3(blocks, 2u * c.kvh, n), kKvThreads, A, s);
 }
 
 int kv8_attend(Kv8AttnArgs& A, const Kv8Plan& P, void* workspace, uint32_t n, hipStream_t s) {
@@ -1278,9 +1435,8 @@ int kv8_attend(Kv8AttnArgs& A, const Kv8Plan& P, void* workspace, uint32_t n, hi
     auto* extra = reinterpret_cast<float*>(ws + P.part + P.ml);
     A.scores = scored && !A.prompt ? extra : nullptr;
     A.stats = scored && A.prompt ? reinterpret_cast<float2*>(extra) : nullptr;
-    const uint32_t nt = A.c.hdp / 32u;
-    const dim3 grid = A.prompt ? dim3((P.units + 3u) / 4u * A.splits * A.c.kvh * n) : dim3(P.units * A.splits, A.c.kvh, n);
-    if (int rc = launch(attn_kernel(nt, cap, A.prompt ? 1 : 0), grid, kKvThreads, A, s)) return rc;
+    if (int rc = launch(kernel_of(A.c, A.prompt ? kKvPrompt : kKvToken, cap), dim3(P.units * A.splits * A.c.kvh * n), kKvThreads, A, s))
+        return rc;
     uint32_t len = 0;
     for (uint32_t i = 0; i < n; ++i)
         if (A.s[i].n) len = std::max(len, A.s[i].pos + A.s[i].n);
@@ -1288,7 +1444,7 @@ int kv8_attend(Kv8AttnArgs& A, const Kv8Plan& P, void* workspace, uint32_t n, hi
     if (wgs)
         if (int rc = launch(reinterpret_cast<const void*>(&k_kv8_join), dim3(wgs, A.c.kvh, n), kKvThreads, A, s)) return rc;
     if (!scored || !A.prompt) return VRT_OK;
-    return launch(attn_kernel(nt, cap, 2), dim3((len + 31u) / 32u, A.c.kvh, n), kKvThreads, A, s);
+    return launch(kernel_of(A.c, kKvWeights, cap), dim3((len + 31u) / 32u, A.c.kvh, n), kKvThreads, A, s);
 }
 
 int kv8_evict(const Kv8Dev& c, const vrt_kv8_move* moves, uint32_t n, float* weights, uint32_t max_ctx, uint32_t* kept,
@@ -1306,7 +1462,7 @@ int kv8_evict(const Kv8Dev& c, const vrt_kv8_move* moves, uint32_t n, float* wei
     }
     if (keep == 0u) return VRT_OK;
     if (int rc = launch(reinterpret_cast<const void*>(&k_kv8_select), dim3(c.kvh, n), kKvSelThreads, A, s)) return rc;
-    return launch(reinterpret_cast<const void*>(&k_kv8_gather), dim3((keep + 31u) / 32u, 2u * c.kvh, n), kKvThreads, A, s);
+    return launch(kernel_of(c, kKvGather), dim3((keep + 31u) / 32u, 2u * c.kvh, n), kKvThreads, A, s);
 }
 
 }  // namespace vrt
@@ -1369,7 +1525,7 @@ extern "C" int vrt_kv8_read(vrt_ctx* ctx, const vrt_kv8_cache* cache, const vrt_
     if (blocks == 0u) return VRT_OK;
     OnDevice on(ctx->device);
     VRT_HIP_CHECK(on.err);
-    return launch(reinterpret_cast<const void*>(&k_kv8_read), dim3(blocks, 2u * A.c.kvh, n_seqs), kKvThreads, A, ctx->stream);
+    return launch(kernel_of(A.c, kKvRead), dim3(blocks, 2u * A.c.kvh, n_seqs), kKvThreads, A, ctx->stream);
 }
 
 extern "C" int vrt_kv8_attend_workspace(const vrt_kv8_cache* cache, const vrt_kv8_attn* attn, const vrt_kv8_rows* rows,

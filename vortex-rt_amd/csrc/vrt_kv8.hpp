@@ -68,7 +68,7 @@ struct Kv8AttnArgs {
     float* w_out;
     uint32_t heads, G, window, max_ctx;
     uint32_t unit;        // rows that run together: 16 (single tokens: a workgroup's waves share them), or a wave's own (prompt)
-    uint32_t prompt, lines;   // lines: rows of a place in the workspace
+    uint32_t prompt, fold, lines;   // fold: all units run at once; lines: rows of a place in the workspace
     uint32_t per, splits; // blocks of a split; the most splits of a sequence
     uint32_t nseq, rows_most;   // rows_most: the most rows (queries times the heads of a group) of a sequence
     float scale, cap;
