@@ -51,12 +51,14 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {   // wave-uniform
     return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), 63));
 }
 
-// x = hi + lo in f16 (x below 2^15 in magnitude; what is lost is below 2^-24)
-__device__ __forceinline__ void kv_split(float x, _Float16& hi, _Float16& lo) {
-    asm("" : "+v"(x));
-    hi = static_cast<_Float16>(x);
-    lo = static_cast<_Float16>(x - static_cast<float>(hi));
+// Pairs of floats to pairs of halves, hi + lo = x (below 2^15 in magnitude; what is lost is below 2^-24). The barrier: see gm_split.
+__device__ __forceinline__ void kv_split2(float x, float y, h2& hi, h2& lo) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    asm("" : "+v"(x), "+v"(y));
+    hi = __builtin_convertvector((f2{x, y}), h2);
+    lo = __builtin_convertvector((f2{x - static_cast<float>(hi[0]), y - static_cast<float>(hi[1])}), h2);
 }
+
 // The exponent e with m 2^e in [2^(to - 1), 2^to), at most 126 so that 2^-e is a number; 0 where m is 0 or not finite.
 __device__ __forceinline__ int kv_exp(float m, int to) {
     return m > 0.0f && m < INFINITY ? min(to - __builtin_amdgcn_frexp_expf(m), 126) : 0;
@@ -90,19 +92,29 @@ __device__ __forceinline__ void kv_unit(uint32_t k, uint32_t& t, uint32_t& d) {
 }
 __device__ __forceinline__ uint32_t f_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
+// Largest magnitudes of the tile's rows, as integers: larger is larger, NaN above infinity above the rest. (Eight neighbouring
+// lanes have the same row.)
 template <int NT>
-__device__ __forceinline__ void kv_close_block(const Kv8Dev& c, const KvTile<NT>& x, uint64_t block, uint32_t z, uint8_t* img,
-                                               uint32_t* red) {
-    const uint32_t tid = threadIdx.x;
-    uint32_t m = 0u;   // |x| as integers: larger is larger, NaN above infinity above the rest
-#pragma unroll
-    for (int k = 0; k < NT; ++k)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) m = max(m, f_bits(x.v[k][e]));
-    m = wave_max_u32(m);
-    if ((tid & 63u) == 0u) red[tid >> 6] = m;
+__device__ __forceinline__ void kv_row_max(const KvTile<NT>& x, uint32_t* rowmax) {
+    if (threadIdx.x < 32u) rowmax[threadIdx.x] = 0u;
     __syncthreads();
-    m = max(max(red[0], red[1]), max(red[2], red[3]));
+#pragma unroll
+    for (int k = 0; k < NT; ++k) {
+        uint32_t t, d, m = max(max(f_bits(x.v[k][0]), f_bits(x.v[k][1])), max(f_bits(x.v[k][2]), f_bits(x.v[k][3])));
+        m = dpp_max_u32<0xB1, 0xf>(m);
+        m = dpp_max_u32<0x4E, 0xf>(m);
+        m = dpp_max_u32<0x141, 0xf>(m);
+        kv_unit<NT>(k, t, d);
+        if ((threadIdx.x & 7u) == 0u) atomicMax(&rowmax[t], m);
+    }
+    __syncthreads();
+}
+
+// A full block's codes and scale.
+template <int NT>
+__device__ __forceinline__ void kv_close_block(const Kv8Dev& c, const KvTile<NT>& x, const uint32_t* rowmax, uint64_t block, uint32_t z,
+                                               uint8_t* img) {
+    const uint32_t tid = threadIdx.x, m = wave_max_u32(rowmax[tid & 31u]);
     const float s = m >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __uint_as_float(m) / 127.0f;
     uint32_t w[NT];
 #pragma unroll
@@ -146,56 +158,47 @@ __device__ __forceinline__ void kv_close_block(const Kv8Dev& c, const KvTile<NT>
     if (tid == 0u) reinterpret_cast<float*>(c.scales + block)[z] = s;
 }
 
-// A tail row, held by a wave (lane l: dims 4 l ..): the fp32 row, and its pair of halves in operand order. The halves of a row
+// Rows r0 .. r1 - 1 of the tile into a tail buffer: the fp32 row, and its pair of halves in operand order. The halves of a row
 // with a value that is not finite are zeros, so that what is masked adds nothing; its factor says so.
-__device__ __forceinline__ void kv_store_tail(const Kv8Dev& c, uint64_t buf, uint32_t z, uint32_t t, f4 v, bool rows) {
-    const uint32_t lane = threadIdx.x & 63u, d = 4u * lane;
-    const uint32_t m = wave_max_u32(max(max(f_bits(v[0]), f_bits(v[1])), max(f_bits(v[2]), f_bits(v[3]))));
-    const bool ok = m < 0x7f800000u;
-    const int ex = kv_exp(__uint_as_float(m), 7);
-    if (lane == 0u) c.factor[buf * 32u + t] = ok ? ldexpf(1.0f, -ex) : __uint_as_float(0x7fc00000u);
-    if (d >= c.hdp) return;
-    if (rows) *reinterpret_cast<f4*>(c.tail + (buf * 32u + t) * c.hdp + d) = v;
+template <int NT>
+__device__ __forceinline__ void kv_store_tail(const Kv8Dev& c, const KvTile<NT>& x, const uint32_t* rowmax, uint64_t buf, uint32_t z,
+                                              uint32_t r0, uint32_t r1) {
     typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-    h4 hi, lo;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        _Float16 a, b;
-        kv_split(ok ? ldexpf(v[e], ex) : 0.0f, a, b);
-        hi[e] = a;
-        lo[e] = b;
+    _Float16* const dst = c.pairs + buf * 64u * c.hdp;
+    if (threadIdx.x >= r0 && threadIdx.x < r1) {
+        const uint32_t m = rowmax[threadIdx.x];
+        c.factor[buf * 32u + threadIdx.x] = m < 0x7f800000u ? ldexpf(1.0f, -kv_exp(__uint_as_float(m), 7)) : __uint_as_float(0x7fc00000u);
     }
-    _Float16* dst = c.pairs + buf * 64u * c.hdp;
-    if (z == 0u) {
-        const uint32_t o = ((d >> 5) * 2u + (t >> 4)) * 512u + (((d >> 3) & 3u) * 16u + (t & 15u)) * 8u + (d & 7u);
-        *reinterpret_cast<h4*>(dst + o) = hi;
-        *reinterpret_cast<h4*>(dst + 32u * c.hdp + o) = lo;
-    } else {
 #pragma unroll
-        for (uint32_t e = 0; e < 4u; ++e) {
-            const uint32_t o = ((d + e) >> 4) * 512u + (((t >> 2) & 3u) * 16u + ((d + e) & 15u)) * 8u + (t & 3u) + (t >> 4) * 4u;
-            dst[o] = hi[e];
-            dst[32u * c.hdp + o] = lo[e];
+    for (int k = 0; k < NT; ++k) {
+        uint32_t t, d;
+        kv_unit<NT>(k, t, d);
+        if (t < r0 || t >= r1) continue;
+        *reinterpret_cast<f4*>(c.tail + (buf * 32u + t) * c.hdp + d) = x.v[k];
+        const uint32_t m = rowmax[t];
+        const bool ok = m < 0x7f800000u;
+        const float up = ldexpf(1.0f, kv_exp(__uint_as_float(m), 7));
+        h4 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+            h2 a, b;
+            kv_split2(ok ? x.v[k][e] * up : 0.0f, ok ? x.v[k][e + 1] * up : 0.0f, a, b);
+            hi[e] = a[0], hi[e + 1] = a[1];
+            lo[e] = b[0], lo[e + 1] = b[1];
+        }
+        if (z == 0u) {
+            const uint32_t o = ((d >> 5) * 2u + (t >> 4)) * 512u + (((d >> 3) & 3u) * 16u + (t & 15u)) * 8u + (d & 7u);
+            *reinterpret_cast<h4*>(dst + o) = hi;
+            *reinterpret_cast<h4*>(dst + 32u * c.hdp + o) = lo;
+        } else {
+#pragma unroll
+            for (uint32_t e = 0; e < 4u; ++e) {
+                const uint32_t o = ((d + e) >> 4) * 512u + (((t >> 2) & 3u) * 16u + ((d + e) & 15u)) * 8u + (t & 3u) + (t >> 4) * 4u;
+                dst[o] = hi[e];
+                dst[32u * c.hdp + o] = lo[e];
+            }
         }
     }
-}
-
-// Positions first .. last of block b (rows of x, which hold the call's positions from p0 on) into its tail. A wave takes
-// every fourth, all of its rows loaded before the first is stored.
-__device__ __forceinline__ void kv_to_tail(const Kv8Dev& c, uint32_t seq, uint32_t head, uint32_t b, uint32_t z, const float* x,
-                                           uint64_t stride, uint32_t p0, uint32_t first, uint32_t last) {
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    f4 v[8];
-#pragma unroll
-    for (uint32_t k = 0; k < 8u; ++k) {
-        const uint32_t p = min(first + wave + 4u * k, last);
-        v[k] = *reinterpret_cast<const f4*>(x + static_cast<uint64_t>(p - p0) * stride + min(4u * lane, c.hd - 4u));
-        if (4u * lane >= c.hd) v[k] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
-    const uint64_t buf = kv_tail_buf(c, seq, head, b, z);
-#pragma unroll
-    for (uint32_t k = 0; k < 8u; ++k)
-        if (first + wave + 4u * k <= last) kv_store_tail(c, buf, z, (first + wave + 4u * k) & 31u, v[k], true);
 }
 
 struct Kv8AppendArgs {
@@ -205,38 +208,41 @@ struct Kv8AppendArgs {
     Kv8Seq s[kKvMaxSeqs];
 };
 
-// One workgroup per (block the call touches, head and K or V, sequence). A full block's codes; the rows of the last two
-// blocks also go to the tail. The first block's earlier rows come from the tail, which a later block of the same parity
-// overwrites: the first block's workgroup writes that one's rows too, after it has read its own.
+// One workgroup per (block the call touches, head and K or V, sequence): a full block's codes; of the last two blocks, the call's
+// rows into the tail. The first block's earlier rows come from the tail, which a later block of the same parity overwrites:
+// the first block's workgroup does that one too, after its own.
 template <int NT>
 __global__ void __launch_bounds__(kKvThreads) k_kv8_append(const Kv8AppendArgs A) {
     __shared__ __align__(16) uint8_t img[1024 * NT];
-    __shared__ uint32_t red[4];
+    __shared__ uint32_t rowmax[32];
     const Kv8Dev& c = A.c;
     const Kv8Seq& S = A.s[blockIdx.z];
     const uint32_t head = blockIdx.y >> 1, z = blockIdx.y & 1u;
     if (S.n == 0u) return;
-    const uint32_t end = S.pos + S.n, b0 = S.pos >> 5, bl = (end - 1u) >> 5, b = b0 + blockIdx.x;
-    if (b > bl) return;
+    const uint32_t end = S.pos + S.n, b0 = S.pos >> 5, bl = (end - 1u) >> 5;
     const float* x = A.x[z] + static_cast<uint64_t>(S.row0) * A.stride + head * c.hd;
-    if ((b + 1u) * 32u <= end) {
+    // the block of the last two that has the first one's tail, if the first one reads it
+    const uint32_t other = (S.pos & 31u) && bl > b0 + 1u ? bl - ((bl ^ b0) & 1u) : b0;
+    for (uint32_t b = b0 + blockIdx.x; b <= bl; b = other) {
+        if (blockIdx.x && b == other) return;
+        const uint32_t first = max(S.pos, 32u * b), last = min(end, 32u * b + 32u);   // the call's rows
+        const uint64_t buf = kv_tail_buf(c, S.seq, head, b, z);
+        const bool full = (b + 1u) * 32u <= end, tail = b + 1u >= bl;
         KvTile<NT> T;
-        const float* old = c.tail + kv_tail_buf(c, S.seq, head, b, z) * 32u * c.hdp;
+        const float* old = c.tail + buf * 32u * c.hdp;
 #pragma unroll
         for (int k = 0; k < NT; ++k) {
             uint32_t t, d;
             kv_unit<NT>(k, t, d);
-            const uint32_t p = 32u * b + t, dd = min(d, c.hd - 4u);
+            const uint32_t p = min(32u * b + t, last - 1u), dd = min(d, c.hd - 4u);
             T.v[k] = *reinterpret_cast<const f4*>(p < S.pos ? old + t * c.hdp + dd : x + static_cast<uint64_t>(p - S.pos) * A.stride + dd);
             if (d >= c.hd) T.v[k] = f4{0.0f, 0.0f, 0.0f, 0.0f};
         }
-        kv_close_block<NT>(c, T, kv_block(c, S.seq, head, b), z, img, red);   // (its barriers come after every read of the tail)
-    }
-    const bool shared = (S.pos & 31u) != 0u;   // the first block reads its tail
-    for (uint32_t t = bl > b0 ? bl - 1u : bl; t <= bl; ++t) {
-        const bool firsts = t == b0 || (shared && ((t ^ b0) & 1u) == 0u);
-        if (firsts ? b == b0 : b == t)
-            kv_to_tail(c, S.seq, head, t, z, x, A.stride, S.pos, max(S.pos, 32u * t), min(end, 32u * t + 32u) - 1u);
+        kv_row_max<NT>(T, rowmax);   // (its barriers come after every read of the tail)
+        if (full) kv_close_block<NT>(c, T, rowmax, kv_block(c, S.seq, head, b), z, img);
+        if (tail) kv_store_tail<NT>(c, T, rowmax, buf, z, first & 31u, last - 32u * b);
+        if (b != b0 || other == b0) return;
+        __syncthreads();   // the next round's row maxima and image
     }
 }
 
@@ -343,14 +349,6 @@ __device__ __forceinline__ float max_xor32(float v) {
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-// Pairs of floats to pairs of halves, hi + lo = x. (The barrier: see gm_split.)
-__device__ __forceinline__ void kv_split2(float x, float y, h2& hi, h2& lo) {
-    typedef float f2 __attribute__((ext_vector_type(2)));
-    asm("" : "+v"(x), "+v"(y));
-    hi = __builtin_convertvector((f2{x, y}), h2);
-    lo = __builtin_convertvector((f2{x - static_cast<float>(hi[0]), y - static_cast<float>(hi[1])}), h2);
-}
-
 // Queries are the B operand of the transposed scores (lane l: row l % 16, dims 32 s + 8 (l / 16) + e), each row scaled by a power
 // of two to below 2^14 and split into halves: units (s, high or low) of 64 lanes x 16 bytes. One tile of 16 rows stays in
 // registers; of more, which all waves of a workgroup share, they stay in LDS, so that the outputs' registers leave
@@ -359,26 +357,35 @@ template <int NT>
 struct KvQuery {
     h8 q[NT][2];
 };
-// Rows r0 .. r0 + 15; f: a score's factor but for its key's scale (log2 units without a cap).
-template <int NT, bool CAP>
-__device__ __forceinline__ void kv_load_q(const Kv8AttnArgs& A, const Kv8Seq& S, uint32_t kvh, uint32_t r0, KvQuery<NT>& Q, float& f) {
+// Rows r0 .. r0 + 15 as they are; from them the queries and f, a score's factor but for its key's scale (log2 units without a cap).
+template <int NT>
+struct KvRows {
+    f4 x[NT][2];
+};
+template <int NT>
+__device__ __forceinline__ void kv_load_rows(const Kv8AttnArgs& A, const Kv8Seq& S, uint32_t kvh, uint32_t r0, KvRows<NT>& X) {
     const uint32_t lane = threadIdx.x & 63u, R = S.n * A.G, hd = A.c.hd;
     const uint32_t r = min(r0 + (lane & 15u), R - 1u), qi = r / A.G, h = kvh * A.G + (r - qi * A.G);
     const float* src = A.q + (static_cast<uint64_t>(S.row0) + qi) * A.q_stride + h * hd;
-    f4 x[NT][2];
+#pragma unroll
+    for (int s = 0; s < NT; ++s)
+#pragma unroll
+        for (uint32_t j = 0; j < 2u; ++j)
+            X.x[s][j] = *reinterpret_cast<const f4*>(src + min(32u * s + 8u * (lane >> 4) + 4u * j, hd - 4u));
+}
+template <int NT, bool CAP>
+__device__ __forceinline__ void kv_make_q(const Kv8AttnArgs& A, KvRows<NT>& X, KvQuery<NT>& Q, float& f) {
+    const uint32_t lane = threadIdx.x & 63u;
     float m = 0.0f;
 #pragma unroll
     for (int s = 0; s < NT; ++s)
 #pragma unroll
-        for (uint32_t j = 0; j < 2u; ++j) {
-            const uint32_t d = 32u * s + 8u * (lane >> 4) + 4u * j;
-            x[s][j] = *reinterpret_cast<const f4*>(src + min(d, hd - 4u));
-            if (d >= hd) x[s][j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-        }
+        for (uint32_t j = 0; j < 2u; ++j)
+            if (32u * s + 8u * (lane >> 4) + 4u * j >= A.c.hd) X.x[s][j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int s = 0; s < NT; ++s)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(x[s][j >> 2][j & 3]));
+        for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(X.x[s][j >> 2][j & 3]));
     m = max_xor32(max_xor16(m));
     const int ex = kv_exp(m, 14);
     const float sign = A.scale < 0.0f ? -1.0f : 1.0f;   // factors are not negative: the largest score is the largest product
@@ -389,10 +396,16 @@ __device__ __forceinline__ void kv_load_q(const Kv8AttnArgs& A, const Kv8Seq& S,
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
             h2 a, b;
-            kv_split2(x[s][j >> 2][j & 3] * up, x[s][j >> 2][(j & 3) + 1] * up, a, b);
+            kv_split2(X.x[s][j >> 2][j & 3] * up, X.x[s][j >> 2][(j & 3) + 1] * up, a, b);
             Q.q[s][0][j] = a[0], Q.q[s][0][j + 1] = a[1];
             Q.q[s][1][j] = b[0], Q.q[s][1][j + 1] = b[1];
         }
+}
+template <int NT, bool CAP>
+__device__ __forceinline__ void kv_load_q(const Kv8AttnArgs& A, const Kv8Seq& S, uint32_t kvh, uint32_t r0, KvQuery<NT>& Q, float& f) {
+    KvRows<NT> X;
+    kv_load_rows<NT>(A, S, kvh, r0, X);
+    kv_make_q<NT, CAP>(A, X, Q, f);
 }
 
 // What a wave holds of RT tiles of 16 rows (lane l: row l % 16 of each). The outputs are transposed too (dims 16 t + 4 (l / 16) + e), in
@@ -437,22 +450,35 @@ __device__ __forceinline__ void kv_load(const Kv8Dev& c, uint64_t blk, uint32_t 
     for (int t = 0; t < NT; ++t) r.w[t] = src[64 * t];
 }
 
-// Products of 32 tokens' keys with the queries: s[k][half], lane l: row l % 16, tokens 16 half + 4 (l / 16) + e.
+// Products of 32 tokens' keys with the queries: s[k][half], lane l: row l % 16, tokens 16 half + 4 (l / 16) + e. Queries in
+// LDS are read kAhead steps (a step: the high or low halves of 32 dims) before their products.
 template <int NT, int RT>
 __device__ __forceinline__ void kv_scores(const KvRaw<NT>& K, const KvWave<NT, RT>& W, f4 (&s)[RT][2]) {
+    constexpr int kAhead = RT == 1 ? 0 : RT == 2 ? 2 : 1;
+    h8 q[kAhead + 1][RT];
 #pragma unroll
     for (int k = 0; k < RT; ++k) s[k][0] = s[k][1] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const h8 a0 = kv_halves(K.w[t].x, K.w[t].y), a1 = kv_halves(K.w[t].z, K.w[t].w);
+    for (int i = 0; i < kAhead; ++i)
 #pragma unroll
-        for (int part = 0; part < 2; ++part)
+        for (int k = 0; k < RT; ++k) q[i][k] = W.query(k, i >> 1, i & 1);
+    h8 a0, a1;
 #pragma unroll
-            for (int k = 0; k < RT; ++k) {
-                const h8 q = W.query(k, t, part);
-                s[k][0] = KV_MFMA(a0, q, s[k][0]);
-                s[k][1] = KV_MFMA(a1, q, s[k][1]);
-            }
+    for (int i = 0; i < 2 * NT; ++i) {
+        const int j = i + kAhead;
+        if (j < 2 * NT)
+#pragma unroll
+            for (int k = 0; k < RT; ++k) q[j % (kAhead + 1)][k] = W.query(k, j >> 1, j & 1);
+        if (RT > 1) __builtin_amdgcn_sched_barrier(0);
+        if ((i & 1) == 0) {
+            a0 = kv_halves(K.w[i >> 1].x, K.w[i >> 1].y);
+            a1 = kv_halves(K.w[i >> 1].z, K.w[i >> 1].w);
+        }
+#pragma unroll
+        for (int k = 0; k < RT; ++k) {
+            s[k][0] = KV_MFMA(a0, q[i % (kAhead + 1)][k], s[k][0]);
+            s[k][1] = KV_MFMA(a1, q[i % (kAhead + 1)][k], s[k][1]);
+        }
     }
 }
 // The same of the open block, from the tail's pairs.
@@ -481,68 +507,71 @@ __device__ __forceinline__ void kv_scores_open(const Kv8Dev& c, uint64_t buf, co
 __device__ __forceinline__ uint32_t kv_token(uint32_t e) { return 4u * ((threadIdx.x & 63u) >> 4) + (e & 3u) + 16u * (e >> 2); }
 
 // One block's scores to weights: log2 units, running reference maximum and sum, the weights times the values' scale as
-// pairs of halves. ks / vs: the block's scales, or (OPEN) those of the lane's tokens. dump: where
-// the row's scores go.
+// pairs of halves. ks / vs: the block's scales, or (OPEN, always masked) those of the lane's tokens. dump: where the row's scores
+// go. Nothing but short pieces is under a condition: what is not seen becomes -infinity, which a factor above zero
+// leaves alone, and a weight of 0; a scale that is NaN becomes a NaN in the sums of the rows that see its block.
 template <int NT, int RT, bool CAP, bool OPEN>
 __device__ __forceinline__ void kv_soft(const Kv8AttnArgs& A, const Kv8Seq& S, uint32_t b, bool masked, f4 (&s)[RT][2],
                                         const float* ks, const float* vs, KvWave<NT, RT>& W, h8 (&ph)[RT], h8 (&pl)[RT], float* dump) {
-    float F[RT], top[RT];   // a score in log2 units is s F (but for a cap or an open block: s is that already)
-    uint32_t see[RT];              // bit e
-    const bool direct = CAP || OPEN;
-    bool some = false;
+    constexpr bool direct = CAP || OPEN;   // s becomes the score itself; else it is s F
+    float F[RT];
 #pragma unroll
-    for (int k = 0; k < RT; ++k) {
-        see[k] = 0xffu;
-        if (masked) {
-            see[k] = 0u;
-            const uint32_t len = S.pos + S.n;
+    for (int k = 0; k < RT; ++k) F[k] = OPEN ? W.f[k] : fmaxf(W.f[k] * ks[0], 1e-36f);
+    if constexpr (OPEN) {
 #pragma unroll
-            for (uint32_t e = 0; e < 8u; ++e) {
-                const uint32_t j = 32u * b + kv_token(e);
-                const bool y = j < len && (j < S.prefix || (j <= W.p[k] && (!A.window || W.p[k] - j < A.window)));
-                see[k] |= static_cast<uint32_t>(y) << e;
-            }
-        }
-        F[k] = OPEN ? W.f[k] : W.f[k] * ks[0];
-        if constexpr (direct) {
-            const float rc = CAP ? 1.0f / A.cap : 1.0f;
+        for (int k = 0; k < RT; ++k)
 #pragma unroll
-            for (uint32_t e = 0; e < 8u; ++e) {
-                float x = s[k][e >> 2][e & 3u];
-                x *= OPEN ? F[k] * ks[e] : F[k];
-                if constexpr (CAP) {
-                    x *= rc;
-                    some |= fabsf(x) > 0.5f;
-                }
-                s[k][e >> 2][e & 3u] = x;
-            }
-        }
+            for (uint32_t e = 0; e < 8u; ++e) s[k][e >> 2][e & 3u] *= F[k] * ks[e];
     }
     if constexpr (CAP) {
+        const float rc = 1.0f / A.cap;
+        bool some = false;
+#pragma unroll
+        for (int k = 0; k < RT; ++k)
+#pragma unroll
+            for (uint32_t e = 0; e < 8u; ++e) {
+                const float x = s[k][e >> 2][e & 3u] * (OPEN ? rc : F[k] * rc);
+                s[k][e >> 2][e & 3u] = x;
+                some |= fabsf(x) > 0.5f;
+            }
         some = __any(some);
 #pragma unroll
         for (int k = 0; k < RT; ++k)
 #pragma unroll
             for (uint32_t e = 0; e < 8u; ++e) s[k][e >> 2][e & 3u] = A.cap * 1.4426950409f * kv_tanh(s[k][e >> 2][e & 3u], some);
     }
-    float v = OPEN ? 0.0f : vs[0];
+    if (masked) {
+        const uint32_t len = S.pos + S.n;
+#pragma unroll
+        for (int k = 0; k < RT; ++k)
+#pragma unroll
+            for (uint32_t e = 0; e < 8u; ++e) {
+                const uint32_t j = 32u * b + kv_token(e);
+                const bool y = j < len && (j < S.prefix || (j <= W.p[k] && (!A.window || W.p[k] - j < A.window)));
+                s[k][e >> 2][e & 3u] = y ? s[k][e >> 2][e & 3u] : -INFINITY;
+            }
+    }
+    float top[RT], v = OPEN ? 0.0f : vs[0];
     if constexpr (OPEN) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v = fmaxf(v, vs[e]);
         v = max_xor32(max_xor16(v));
+    } else if (!(ks[0] < INFINITY) || !(v < INFINITY)) {   // the block stands for NaN
+        v = 0.0f;
+#pragma unroll
+        for (int k = 0; k < RT; ++k)
+#pragma unroll
+            for (uint32_t e = 0; e < 8u; ++e) W.l[k] = s[k][e >> 2][e & 3u] != -INFINITY ? __uint_as_float(0x7fc00000u) : W.l[k];
     }
-    const int ev = v > 0.0f && v < INFINITY ? __builtin_amdgcn_frexp_expf(v) : kKvNoExp;
+    const int ev = v > 0.0f ? __builtin_amdgcn_frexp_expf(v) : kKvNoExp;
     bool grow = ev > W.eR;
 #pragma unroll
     for (int k = 0; k < RT; ++k) {
-        if (masked)
-#pragma unroll
-            for (uint32_t e = 0; e < 8u; ++e) s[k][e >> 2][e & 3u] = (see[k] >> e) & 1u ? s[k][e >> 2][e & 3u] : -INFINITY;
         float t = -INFINITY;
 #pragma unroll
         for (uint32_t e = 0; e < 8u; ++e) t = fmaxf(t, s[k][e >> 2][e & 3u]);
         t = max_xor32(max_xor16(t));
-        top[k] = direct || t == -INFINITY ? t : t * F[k];
+        top[k] = direct ? t : t * F[k];
         grow |= top[k] > W.m[k] + kKvGrow;
     }
     if (__any(grow)) {
@@ -562,7 +591,7 @@ __device__ __forceinline__ void kv_soft(const Kv8AttnArgs& A, const Kv8Seq& S, u
         W.eR = eR;
     }
     const int up = W.eR == kKvNoExp ? 0 : 9 - W.eR;
-    const float vf = OPEN ? 0.0f : ldexpf(vs[0], up);
+    const float vf = ldexpf(v, up);
 #pragma unroll
     for (int k = 0; k < RT; ++k) {
         const float ref = W.m[k] == -INFINITY ? 0.0f : W.m[k];
@@ -571,10 +600,9 @@ __device__ __forceinline__ void kv_soft(const Kv8AttnArgs& A, const Kv8Seq& S, u
         for (uint32_t e = 0; e < 8u; ++e) {
             const float x = s[k][e >> 2][e & 3u];
             p[e] = __builtin_amdgcn_exp2f(direct ? x - ref : __builtin_fmaf(x, F[k], -ref));
-            if (masked) p[e] = (see[k] >> e) & 1u ? p[e] : 0.0f;
             W.l[k] += p[e];
-            p[e] *= OPEN ? ldexpf(vs[e], up) : vf;
-            if (masked) p[e] = (see[k] >> e) & 1u ? p[e] : 0.0f;   // (0 times a scale that is NaN)
+            if constexpr (OPEN) p[e] = x == -INFINITY ? 0.0f : p[e] * ldexpf(vs[e], up);   // (0 times a factor that is NaN)
+            else p[e] *= vf;
         }
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
@@ -587,10 +615,7 @@ __device__ __forceinline__ void kv_soft(const Kv8AttnArgs& A, const Kv8Seq& S, u
     if (dump) {
         f4 x[2];
 #pragma unroll
-        for (uint32_t e = 0; e < 8u; ++e) {
-            const float y = s[0][e >> 2][e & 3u];
-            x[e >> 2][e & 3u] = direct || y == -INFINITY ? y : y * F[0];
-        }
+        for (uint32_t e = 0; e < 8u; ++e) x[e >> 2][e & 3u] = s[0][e >> 2][e & 3u] * (direct ? 1.0f : F[0]);
         *reinterpret_cast<f4*>(dump) = x[0];
         *reinterpret_cast<f4*>(dump + 16) = x[1];
     }
@@ -682,7 +707,8 @@ __device__ __forceinline__ void kv_row_done(const Kv8AttnArgs& A, uint32_t row, 
 }
 
 // The virtual blocks i0, i0 + 4, ... below i1 of a wave's rows (span sp). The keys of the next block are loaded while
-// this one's weights are computed, its values while the next scores are; the first block's before start() makes the queries.
+// this one's weights are computed, its values while the next scores are (several tiles, whose blocks come out of L2: after the
+// scores, which leaves those registers to the queries); the first block's before start() makes the queries.
 template <int NT, int RT, bool CAP, class Start>
 __device__ __forceinline__ void kv_run(const Kv8AttnArgs& A, const Kv8Seq& S, uint32_t kvh, const KvSpan& sp, uint32_t pmin, uint32_t pmax,
                                        uint32_t i0, uint32_t i1, KvWave<NT, RT>& W, float* dump, Start start) {
@@ -697,7 +723,7 @@ __device__ __forceinline__ void kv_run(const Kv8AttnArgs& A, const Kv8Seq& S, ui
     // (a wave without a full block loads one all the same, the first of the region, and uses nothing of it)
     uint64_t blk = kv_block(c, S.seq, kvh, any ? block(i0) : 0u);
     kv_load<NT>(c, blk, 0u, K);
-    kv_load<NT>(c, blk, 1u, V);
+    if (RT == 1) kv_load<NT>(c, blk, 1u, V);
     sc = c.scales[blk];
     __builtin_amdgcn_sched_barrier(0);
     start();
@@ -706,6 +732,7 @@ __device__ __forceinline__ void kv_run(const Kv8AttnArgs& A, const Kv8Seq& S, ui
         const uint32_t b = block(i);
         f4 s[RT][2];
         kv_scores<NT, RT>(K, W, s);
+        if (RT > 1) kv_load<NT>(c, blk, 1u, V);
         // (the last block's "next" is itself, again in cache: with no branch, a wait counts the loads it is for alone)
         blk = kv_block(c, S.seq, kvh, block(i + 4u < e1 ? i + 4u : i));
         kv_load<NT>(c, blk, 0u, K);
@@ -716,7 +743,7 @@ __device__ __forceinline__ void kv_run(const Kv8AttnArgs& A, const Kv8Seq& S, ui
         kv_soft<NT, RT, CAP, false>(A, S, b, kv_masked(A, S, b, pmin, pmax), s, &cur.x, &cur.y, W, ph, pl,
                                     dump ? dump + 32u * (i - i0) : nullptr);
         kv_values<NT, RT>(V, ph, pl, W);
-        kv_load<NT>(c, blk, 1u, V);
+        if (RT == 1) kv_load<NT>(c, blk, 1u, V);
         __builtin_amdgcn_sched_barrier(0);
     }
     if (open && i == sp.n - 1u && i < i1) kv_open<NT, RT, CAP>(A, S, kvh, last, W, dump ? dump + 32u * (i - i0) : nullptr);
@@ -900,45 +927,63 @@ __global__ void __launch_bounds__(kKvThreads) k_kv8_join(const Kv8AttnArgs A) {
     A.w_out[at] = (A.w_in && j < S.pos ? A.w_in[at] : 0.0f) + w;
 }
 
-// Prompts' accumulated weights: one workgroup per (block of positions, head, sequence), its waves taking every fourth tile of 16
-// rows; the scores once more, against the rows' final maxima and sums.
+// Prompts' accumulated weights: one workgroup per (block of positions, head, sequence), its waves taking every eighth of the 16-row
+// tiles that see the block; the scores once more, against the rows' final maxima and sums. A tile's rows are loaded while the
+// one before is worked on.
+constexpr uint32_t kKvWeightWaves = 8;
 template <int NT, bool CAP>
-__global__ void __launch_bounds__(kKvThreads, 2) k_kv8_weights(const Kv8AttnArgs A) {
-    __shared__ float s_w[4][32];
+__global__ void __launch_bounds__(64 * kKvWeightWaves, 2) k_kv8_weights(const Kv8AttnArgs A) {
+    __shared__ float s_w[kKvWeightWaves][32];
     const Kv8Seq& S = A.s[blockIdx.z];
     const Kv8Dev& c = A.c;
     const uint32_t kvh = blockIdx.y, m16 = threadIdx.x & 15u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t len = S.pos + S.n, R = S.n * A.G, b = blockIdx.x;
-    if (S.n == 0u || 32u * b >= len) return;
-    const bool open = (b + 1u) * 32u > len, in_pre = 32u * b < S.prefix;
+    const uint32_t len = S.pos + S.n, R = S.n * A.G, b = blockIdx.x, p0 = 32u * b, p1 = p0 + 31u;
+    if (S.n == 0u || p0 >= len) return;
+    const bool open = p1 >= len;
     float w[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
     float ks[8];
     KvRaw<NT> K;
     const uint64_t kb = kv_tail_buf(c, S.seq, kvh, b, 0u);
     if (open) {
 #pragma unroll
-        for (uint32_t e = 0; e < 8u; ++e) ks[e] = 32u * b + kv_token(e) < len ? c.factor[kb * 32u + kv_token(e)] : 0.0f;
+        for (uint32_t e = 0; e < 8u; ++e) ks[e] = p0 + kv_token(e) < len ? c.factor[kb * 32u + kv_token(e)] : 0.0f;
     } else {
         const uint64_t blk = kv_block(c, S.seq, kvh, b);
         kv_load<NT>(c, blk, 0u, K);
 #pragma unroll
         for (int e = 0; e < 8; ++e) ks[e] = c.scales[blk].x;
     }
-    for (uint32_t r0 = 16u * wave; r0 < R; r0 += 64u) {
+    // the tiles that see the block: all of a prefix's, else from its first position's query to the last within the window
+    uint32_t t0 = 0u, t1 = (R + 15u) / 16u;
+    if (p0 >= S.prefix) {
+        if (p0 > S.pos) t0 = (p0 - S.pos) * A.G / 16u;
+        if (A.window && p1 + A.window > p1) {   // (query p1 + window - 1)
+            const uint32_t q1 = p1 + A.window;
+            t1 = q1 <= S.pos ? 0u : min(t1, static_cast<uint32_t>((static_cast<uint64_t>(q1 - S.pos) * A.G + 15u) / 16u));
+        }
+    }
+    KvRows<NT> X;
+    float2 st_next;
+    auto fetch = [&](uint32_t t) {
+        kv_load_rows<NT>(A, S, kvh, 16u * t, X);
+        const uint32_t r = min(16u * t + m16, R - 1u), qi = r / A.G;
+        st_next = A.stats[(static_cast<uint64_t>(S.row0) + qi) * A.heads + kvh * A.G + (r - qi * A.G)];
+    };
+    uint32_t t = t0 + wave;
+    if (t < t1) fetch(t);
+    for (; t < t1; t += kKvWeightWaves) {
+        const uint32_t r0 = 16u * t, r = r0 + m16, p = S.pos + min(r, R - 1u) / A.G;
         const uint32_t pmin = S.pos + r0 / A.G, pmax = S.pos + min(r0 + 15u, R - 1u) / A.G;
-        if (!in_pre && 32u * b > pmax) continue;
-        if (!in_pre && A.window && pmin >= A.window && 32u * b + 31u <= pmin - A.window) break;   // and no later row sees it
         KvWave<NT, 1> W;
-        kv_load_q<NT, CAP>(A, S, kvh, r0, W.q, W.f[0]);
+        kv_make_q<NT, CAP>(A, X, W.q, W.f[0]);
+        const float2 st = st_next;
+        fetch(min(t + kKvWeightWaves, t1 - 1u));
+        __builtin_amdgcn_sched_barrier(0);
         f4 s[1][2];
         if (open) kv_scores_open<NT, 1>(c, kb, W, s);
         else kv_scores<NT, 1>(K, W, s);
-        const uint32_t r = r0 + m16;
         const bool masked = open || r0 + 15u >= R || kv_masked(A, S, b, pmin, pmax);
-        const uint32_t qi = min(r, R - 1u) / A.G, h = kvh * A.G + (min(r, R - 1u) - qi * A.G);
-        const float2 st = A.stats[(static_cast<uint64_t>(S.row0) + qi) * A.heads + h];
-        const uint32_t p0 = S.pos + qi;
         float x[8];
         bool some = false;
 #pragma unroll
@@ -955,27 +1000,30 @@ __global__ void __launch_bounds__(kKvThreads, 2) k_kv8_weights(const Kv8AttnArgs
             for (int e = 0; e < 8; ++e) x[e] = A.cap * 1.4426950409f * kv_tanh(x[e], some);
         }
 #pragma unroll
-        for (uint32_t e = 0; e < 8u; ++e) {
-            float p = __builtin_amdgcn_exp2f(x[e] - st.x) * st.y;
-            if (masked) {
-                const uint32_t j = 32u * b + kv_token(e);
-                const bool y = r < R && j < len && (j < S.prefix || (j <= p0 && (!A.window || p0 - j < A.window)));
-                p = y ? p : 0.0f;
+        for (uint32_t e = 0; e < 8u; ++e) x[e] = __builtin_amdgcn_exp2f(x[e] - st.x) * st.y;
+        if (masked)
+#pragma unroll
+            for (uint32_t e = 0; e < 8u; ++e) {
+                const uint32_t j = p0 + kv_token(e);
+                const bool y = r < R && j < len && (j < S.prefix || (j <= p && (!A.window || p - j < A.window)));
+                x[e] = y ? x[e] : 0.0f;
             }
-            w[e] += p;
-        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] += x[e];
     }
 #pragma unroll
     for (uint32_t e = 0; e < 8u; ++e) {
-        const float t = slot_sum<16>(w[e]);
-        if (m16 == 0u) s_w[wave][kv_token(e)] = t;
+        const float y = slot_sum<16>(w[e]);
+        if (m16 == 0u) s_w[wave][kv_token(e)] = y;
     }
     __syncthreads();
-    const uint32_t j = 32u * b + threadIdx.x;
+    const uint32_t j = p0 + threadIdx.x;
     if (threadIdx.x >= 32u || j >= len) return;
-    const float t = (s_w[0][threadIdx.x] + s_w[1][threadIdx.x]) + (s_w[2][threadIdx.x] + s_w[3][threadIdx.x]);
+    float y = 0.0f;
+#pragma unroll
+    for (uint32_t v = 0; v < kKvWeightWaves; ++v) y += s_w[v][threadIdx.x];
     const uint64_t at = (static_cast<uint64_t>(S.seq) * c.kvh + kvh) * A.max_ctx + j;
-    A.w_out[at] = (A.w_in && j < S.pos ? A.w_in[at] : 0.0f) + t;
+    A.w_out[at] = (A.w_in && j < S.pos ? A.w_in[at] : 0.0f) + y;
 }
 
 // ---- eviction -------------------------------------------------------------------------------
@@ -1015,7 +1063,7 @@ __global__ void __launch_bounds__(kKvSelThreads) k_kv8_select(const Kv8EvictArgs
     if (want == 0u) return;
     uint32_t thr = 0u, need = want;   // keys above thr stay, and `need` of those equal to it
     constexpr uint32_t kShift[3] = {21u, 10u, 0u}, kBits[3] = {11u, 11u, 10u};
-    constexpr uint32_t kAhead = 8u;   // loads in flight
+    constexpr uint32_t kAhead = 16u;   // loads in flight
 #pragma unroll
     for (int pass = 0; pass < 3; ++pass) {
         const uint32_t shift = kShift[pass], mask = (1u << kBits[pass]) - 1u, high = pass == 0 ? 0u : 0xffffffffu << (shift + kBits[pass]);
@@ -1031,11 +1079,13 @@ __global__ void __launch_bounds__(kKvSelThreads) k_kv8_select(const Kv8EvictArgs
                 const bool in = i0 + kKvSelThreads * k < old && (key & high) == thr;
                 const uint64_t all = __ballot(in);
                 if (!all) continue;
-                // lanes with the same bin as the first of them (often all) add once
+                // (lanes of one bin add one after the other: where all have the same, as where weights are 0, one adds for them)
                 const uint32_t first = __builtin_amdgcn_readlane(static_cast<int>(bin), __builtin_ctzll(all));
-                const uint64_t same = __ballot(in && bin == first);
-                if (lane == static_cast<uint32_t>(__builtin_ctzll(same))) atomicAdd(&hist[first], static_cast<uint32_t>(__popcll(same)));
-                if (in && bin != first) atomicAdd(&hist[bin], 1u);
+                if (__ballot(in && bin == first) == all) {
+                    if (lane == static_cast<uint32_t>(__builtin_ctzll(all))) atomicAdd(&hist[first], static_cast<uint32_t>(__popcll(all)));
+                } else if (in) {
+                    atomicAdd(&hist[bin], 1u);
+                }
             }
         }
         __syncthreads();
@@ -1113,7 +1163,7 @@ __global__ void __launch_bounds__(kKvThreads) k_kv8_gather(const Kv8EvictArgs A)
     constexpr uint32_t kRow = 32u * NT + 8u;
     __shared__ __align__(16) uint8_t img[1024 * NT];
     __shared__ __align__(16) uint8_t raw[32 * kRow];
-    __shared__ uint32_t red[4], s_p[32];
+    __shared__ uint32_t rowmax[32], s_p[32];
     __shared__ float s_s[32];
     const Kv8Dev& c = A.c;
     const vrt_kv8_move& V = A.m[blockIdx.z];
@@ -1127,28 +1177,39 @@ __global__ void __launch_bounds__(kKvThreads) k_kv8_gather(const Kv8EvictArgs A)
         s_s[tid] = (p >> 5) < full ? reinterpret_cast<const float*>(c.scales + kv_block(c, V.src, head, p >> 5))[z] : 0.0f;
     }
     __syncthreads();
+    // (every load issued, at a position that is there, before the first is put down)
     if (z == 0u) {
-        for (uint32_t i = tid; i < 128u * NT; i += kKvThreads) {   // (8 dims, token)
-            const uint32_t t = i & 31u, q = i >> 5, p = s_p[t];
-            if ((p >> 5) >= full) continue;
-            const uint8_t* blk = kv_codes(c, kv_block(c, V.src, head, p >> 5));
-            *reinterpret_cast<uint2*>(raw + t * kRow + 8u * q) = *reinterpret_cast<const uint2*>(blk + kv_k_at(p & 31u, 8u * q));
+        constexpr uint32_t kPer = (128u * NT + kKvThreads - 1u) / kKvThreads;
+        uint2 u[kPer];
+#pragma unroll
+        for (uint32_t k = 0; k < kPer; ++k) {   // (8 dims, token)
+            const uint32_t i = min(tid + kKvThreads * k, 128u * NT - 1u), t = i & 31u, q = i >> 5, p = s_p[t];
+            const uint8_t* blk = kv_codes(c, kv_block(c, V.src, head, min(p >> 5, full - 1u)));
+            u[k] = *reinterpret_cast<const uint2*>(blk + kv_k_at(p & 31u, 8u * q));
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < kPer; ++k) {
+            const uint32_t i = min(tid + kKvThreads * k, 128u * NT - 1u), t = i & 31u, q = i >> 5;
+            *reinterpret_cast<uint2*>(raw + t * kRow + 8u * q) = u[k];
         }
     } else {
-        for (uint32_t i = tid; i < 512u * NT; i += kKvThreads) {   // (token, dims 32 jj + m and 16 on)
-            const uint32_t m = i & 15u, jj = (i >> 4) % NT, t = (i >> 4) / NT, p = s_p[t], tok = p & 31u;
-            if ((p >> 5) >= full) continue;
-            const uint8_t* blk = kv_codes(c, kv_block(c, V.src, head, p >> 5)) + 32u * c.hdp;
-            const uint4 u = *reinterpret_cast<const uint4*>(blk + jj * 1024u + (((tok >> 2) & 3u) * 16u + m) * 16u);
+        uint4 u[2 * NT];
+#pragma unroll
+        for (uint32_t k = 0; k < 2u * NT; ++k) {   // (token, dims 32 jj + m and 16 on)
+            const uint32_t i = tid + kKvThreads * k, m = i & 15u, jj = (i >> 4) % NT, t = (i >> 4) / NT, p = s_p[t];
+            const uint8_t* blk = kv_codes(c, kv_block(c, V.src, head, min(p >> 5, full - 1u))) + 32u * c.hdp;
+            u[k] = *reinterpret_cast<const uint4*>(blk + jj * 1024u + (((p >> 2) & 3u) * 16u + m) * 16u);
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < 2u * NT; ++k) {
+            const uint32_t i = tid + kKvThreads * k, m = i & 15u, jj = (i >> 4) % NT, t = (i >> 4) / NT, tok = s_p[t] & 31u;
             const bool late = tok >> 4;
             const uint32_t sh = 8u * (tok & 3u);
-            raw[t * kRow + 32u * jj + m] = static_cast<uint8_t>((late ? u.y : u.x) >> sh);
-            raw[t * kRow + 32u * jj + 16u + m] = static_cast<uint8_t>((late ? u.w : u.z) >> sh);
+            raw[t * kRow + 32u * jj + m] = static_cast<uint8_t>((late ? u[k].y : u[k].x) >> sh);
+            raw[t * kRow + 32u * jj + 16u + m] = static_cast<uint8_t>((late ? u[k].w : u[k].z) >> sh);
         }
     }
     __syncthreads();
-    const bool closed = n == 32u, tail = b + 1u >= (V.keep - 1u) >> 5;   // the last block and the one before
-    const uint64_t buf = kv_tail_buf(c, V.dst, head, b, z);
     KvTile<NT> T;
 #pragma unroll
     for (int k = 0; k < NT; ++k) {
@@ -1164,17 +1225,11 @@ __global__ void __launch_bounds__(kKvThreads) k_kv8_gather(const Kv8EvictArgs A)
         } else {
             T.v[k] = *reinterpret_cast<const f4*>(c.tail + (kv_tail_buf(c, V.src, head, p >> 5, z) * 32u + (p & 31u)) * c.hdp + d);
         }
-        if (tail) *reinterpret_cast<f4*>(c.tail + (buf * 32u + t) * c.hdp + d) = T.v[k];
     }
-    if (closed) kv_close_block<NT>(c, T, kv_block(c, V.dst, head, b), z, img, red);
-    if (!tail) return;
-    __syncthreads();   // the tail's rows are whole: a wave each for their pairs
-    const uint32_t lane = tid & 63u;
-    for (uint32_t t = tid >> 6; t < n; t += kKvThreads / 64u) {
-        f4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (4u * lane < c.hd) v = *reinterpret_cast<const f4*>(c.tail + (buf * 32u + t) * c.hdp + 4u * lane);
-        kv_store_tail(c, buf, z, t, v, false);
-    }
+    kv_row_max<NT>(T, rowmax);
+    if (n == 32u) kv_close_block<NT>(c, T, rowmax, kv_block(c, V.dst, head, b), z, img);
+    if (b + 1u >= (V.keep - 1u) >> 5)   // the last block and the one before
+        kv_store_tail<NT>(c, T, rowmax, kv_tail_buf(c, V.dst, head, b, z), z, 0u, n);
 }
 
 // ---- host -----------------------------------------------------------------------------------
@@ -1444,7 +1499,7 @@ int kv8_attend(Kv8AttnArgs& A, const Kv8Plan& P, void* workspace, uint32_t n, hi
     if (wgs)
         if (int rc = launch(reinterpret_cast<const void*>(&k_kv8_join), dim3(wgs, A.c.kvh, n), kKvThreads, A, s)) return rc;
     if (!scored || !A.prompt) return VRT_OK;
-    return launch(kernel_of(A.c, kKvWeights, cap), dim3((len + 31u) / 32u, A.c.kvh, n), kKvThreads, A, s);
+    return launch(kernel_of(A.c, kKvWeights, cap), dim3((len + 31u) / 32u, A.c.kvh, n), 64u * kKvWeightWaves, A, s);
 }
 
 int kv8_evict(const Kv8Dev& c, const vrt_kv8_move* moves, uint32_t n, float* weights, uint32_t max_ctx, uint32_t* kept,
