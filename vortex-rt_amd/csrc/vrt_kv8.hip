@@ -78,15 +78,17 @@ __device__ __forceinline__ float kv_round(float x, float s, float inv) {
 
 // ---- append ---------------------------------------------------------------------------------
 
-// A workgroup's 32 rows of one head and block: NT float4 a thread (unit tid + 256 k: token unit / (8 NT), dims 4 (unit %
-// (8 NT)) ..; zeros past hd), their largest magnitude, scale, codes, in operand order through an LDS image.
+// A workgroup's 32 rows of one head and block: KU float4 a thread (unit tid + TH k: token unit / (8 NT), dims 4 (unit % (8 NT)) ..;
+// zeros past hd; the last unit again past the end), their largest magnitude, scale, codes, in operand order through an LDS
+// image. Of 96 dims and more, 512 threads: with 256 a thread's share of 256 dims takes 217 registers, or spills.
 template <int NT>
 struct KvTile {
-    f4 v[NT];
+    static constexpr uint32_t TH = NT >= 3 ? 512u : 256u, KU = (256u * NT + TH - 1u) / TH;
+    f4 v[KU];
 };
 template <int NT>
 __device__ __forceinline__ void kv_unit(uint32_t k, uint32_t& t, uint32_t& d) {
-    const uint32_t u = threadIdx.x + kKvThreads * k;
+    const uint32_t u = min(threadIdx.x + KvTile<NT>::TH * k, 256u * NT - 1u);
     t = u / (8u * NT);
     d = (u - t * 8u * NT) * 4u;
 }
@@ -99,7 +101,7 @@ __device__ __forceinline__ void kv_row_max(const KvTile<NT>& x, uint32_t* rowmax
     if (threadIdx.x < 32u) rowmax[threadIdx.x] = 0u;
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < NT; ++k) {
+    for (uint32_t k = 0; k < KvTile<NT>::KU; ++k) {
         uint32_t t, d, m = max(max(f_bits(x.v[k][0]), f_bits(x.v[k][1])), max(f_bits(x.v[k][2]), f_bits(x.v[k][3])));
         m = dpp_max_u32<0xB1, 0xf>(m);
         m = dpp_max_u32<0x4E, 0xf>(m);
@@ -116,15 +118,15 @@ __device__ __forceinline__ void kv_close_block(const Kv8Dev& c, const KvTile<NT>
                                                uint8_t* img) {
     const uint32_t tid = threadIdx.x, m = wave_max_u32(rowmax[tid & 31u]);
     const float s = m >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __uint_as_float(m) / 127.0f;
-    uint32_t w[NT];
+    uint32_t w[KvTile<NT>::KU];
 #pragma unroll
-    for (int k = 0; k < NT; ++k) w[k] = 0x80808080u;
+    for (uint32_t k = 0; k < KvTile<NT>::KU; ++k) w[k] = 0x80808080u;
     if (s > 0.0f) {
         // the quotient's steps stay away from denormals: their halves and reciprocals are no numbers
         const float up = s < 0x1p-100f ? 0x1p60f : 1.0f, su = s * up, inv = 1.0f / su, half = 0.5f * su;
         bool near = false;   // a remainder of half a step or more: the quotient may be one off, or a tie
 #pragma unroll
-        for (int k = 0; k < NT; ++k) {
+        for (uint32_t k = 0; k < KvTile<NT>::KU; ++k) {
             w[k] = 0u;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -135,14 +137,14 @@ __device__ __forceinline__ void kv_close_block(const Kv8Dev& c, const KvTile<NT>
         }
         if (__any(near))   // seldom
 #pragma unroll
-            for (int k = 0; k < NT; ++k) {
+            for (uint32_t k = 0; k < KvTile<NT>::KU; ++k) {
                 w[k] = 0u;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) w[k] = __builtin_amdgcn_cvt_pk_u8_f32(kv_round(x.v[k][e] * up, su, inv) + 128.0f, e, w[k]);
             }
     }
 #pragma unroll
-    for (int k = 0; k < NT; ++k) {
+    for (uint32_t k = 0; k < KvTile<NT>::KU; ++k) {
         uint32_t t, d;
         kv_unit<NT>(k, t, d);
         if (z == 0u) {
@@ -154,50 +156,86 @@ __device__ __forceinline__ void kv_close_block(const Kv8Dev& c, const KvTile<NT>
     }
     __syncthreads();
     uint4* dst = reinterpret_cast<uint4*>(kv_codes(c, block) + z * 32u * c.hdp);
-    for (uint32_t i = tid; i < 64u * NT; i += kKvThreads) dst[i] = reinterpret_cast<const uint4*>(img)[i];
+    for (uint32_t i = tid; i < 64u * NT; i += KvTile<NT>::TH) dst[i] = reinterpret_cast<const uint4*>(img)[i];
     if (tid == 0u) reinterpret_cast<float*>(c.scales + block)[z] = s;
 }
 
-// Rows r0 .. r1 - 1 of the tile into a tail buffer: the fp32 row, and its pair of halves in operand order. The halves of a row
-// with a value that is not finite are zeros, so that what is masked adds nothing; its factor says so.
+constexpr uint32_t kKvFew = 2;   // rows whose pairs are scattered
+
+// Halves of a row's pair in operand order: K by four dims, V by one.
+__device__ __forceinline__ uint32_t kv_k_half(uint32_t t, uint32_t d) {
+    return ((d >> 5) * 2u + (t >> 4)) * 512u + (((d >> 3) & 3u) * 16u + (t & 15u)) * 8u + (d & 7u);
+}
+__device__ __forceinline__ uint32_t kv_v_half(uint32_t t, uint32_t d) {
+    return (d >> 4) * 512u + (((t >> 2) & 3u) * 16u + (d & 15u)) * 8u + (t & 3u) + (t >> 4) * 4u;
+}
+
+// Rows r0 .. r1 - 1 of the tile (which has all rows below r1) into a tail buffer: the fp32 rows, and pairs of halves in operand order.
+// The halves of a row with a value that is not finite are zeros, so that what is masked adds nothing; its factor says so.
+// A few rows' pairs are scattered (a value's halves are 2-byte stores, 16 bytes apart); of more, the whole buffer's go
+// through LDS: scattered, 32 rows of 256 took a workgroup 7 us. img: 2048 NT bytes.
 template <int NT>
 __device__ __forceinline__ void kv_store_tail(const Kv8Dev& c, const KvTile<NT>& x, const uint32_t* rowmax, uint64_t buf, uint32_t z,
-                                              uint32_t r0, uint32_t r1) {
+                                              uint32_t r0, uint32_t r1, uint8_t* img) {
     typedef _Float16 h4 __attribute__((ext_vector_type(4)));
     _Float16* const dst = c.pairs + buf * 64u * c.hdp;
-    if (threadIdx.x >= r0 && threadIdx.x < r1) {
-        const uint32_t m = rowmax[threadIdx.x];
-        c.factor[buf * 32u + threadIdx.x] = m < 0x7f800000u ? ldexpf(1.0f, -kv_exp(__uint_as_float(m), 7)) : __uint_as_float(0x7fc00000u);
+    const uint32_t tid = threadIdx.x;
+    if (tid >= r0 && tid < r1) {
+        const uint32_t m = rowmax[tid];
+        c.factor[buf * 32u + tid] = m < 0x7f800000u ? ldexpf(1.0f, -kv_exp(__uint_as_float(m), 7)) : __uint_as_float(0x7fc00000u);
     }
-#pragma unroll
-    for (int k = 0; k < NT; ++k) {
-        uint32_t t, d;
-        kv_unit<NT>(k, t, d);
-        if (t < r0 || t >= r1) continue;
-        *reinterpret_cast<f4*>(c.tail + (buf * 32u + t) * c.hdp + d) = x.v[k];
+    auto row = [&](uint32_t k, uint32_t t, h4 (&pair)[2]) {
         const uint32_t m = rowmax[t];
-        const bool ok = m < 0x7f800000u;
+        const bool ok = m < 0x7f800000u && t < r1;
         const float up = ldexpf(1.0f, kv_exp(__uint_as_float(m), 7));
-        h4 hi, lo;
 #pragma unroll
         for (int e = 0; e < 4; e += 2) {
             h2 a, b;
             kv_split2(ok ? x.v[k][e] * up : 0.0f, ok ? x.v[k][e + 1] * up : 0.0f, a, b);
-            hi[e] = a[0], hi[e + 1] = a[1];
-            lo[e] = b[0], lo[e + 1] = b[1];
+            pair[0][e] = a[0], pair[0][e + 1] = a[1];
+            pair[1][e] = b[0], pair[1][e + 1] = b[1];
         }
-        if (z == 0u) {
-            const uint32_t o = ((d >> 5) * 2u + (t >> 4)) * 512u + (((d >> 3) & 3u) * 16u + (t & 15u)) * 8u + (d & 7u);
-            *reinterpret_cast<h4*>(dst + o) = hi;
-            *reinterpret_cast<h4*>(dst + 32u * c.hdp + o) = lo;
-        } else {
+    };
+    if (r1 - r0 <= kKvFew) {
 #pragma unroll
-            for (uint32_t e = 0; e < 4u; ++e) {
-                const uint32_t o = ((d + e) >> 4) * 512u + (((t >> 2) & 3u) * 16u + ((d + e) & 15u)) * 8u + (t & 3u) + (t >> 4) * 4u;
-                dst[o] = hi[e];
-                dst[32u * c.hdp + o] = lo[e];
+        for (uint32_t k = 0; k < KvTile<NT>::KU; ++k) {
+            uint32_t t, d;
+            kv_unit<NT>(k, t, d);
+            if (t < r0 || t >= r1) continue;
+            *reinterpret_cast<f4*>(c.tail + (buf * 32u + t) * c.hdp + d) = x.v[k];
+            h4 pair[2];
+            row(k, t, pair);
+#pragma unroll
+            for (uint32_t part = 0; part < 2u; ++part) {
+                _Float16* const to = dst + part * 32u * c.hdp;
+                if (z == 0u) *reinterpret_cast<h4*>(to + kv_k_half(t, d)) = pair[part];
+                else
+#pragma unroll
+                    for (uint32_t e = 0; e < 4u; ++e) to[kv_v_half(t, d + e)] = pair[part][e];
             }
         }
+        return;
+    }
+    _Float16* const im = reinterpret_cast<_Float16*>(img);
+#pragma unroll 1
+    for (uint32_t part = 0; part < 2u; ++part) {
+        __syncthreads();
+#pragma unroll
+        for (uint32_t k = 0; k < KvTile<NT>::KU; ++k) {
+            uint32_t t, d;
+            kv_unit<NT>(k, t, d);
+            if (part == 0u && t >= r0 && t < r1) *reinterpret_cast<f4*>(c.tail + (buf * 32u + t) * c.hdp + d) = x.v[k];
+            h4 pair[2];
+            row(k, t, pair);
+            const h4 v = part ? pair[1] : pair[0];
+            if (z == 0u) *reinterpret_cast<h4*>(im + kv_k_half(t, d)) = v;
+            else
+#pragma unroll
+                for (uint32_t e = 0; e < 4u; ++e) im[kv_v_half(t, d + e)] = v[e];
+        }
+        __syncthreads();
+        uint4* const to = reinterpret_cast<uint4*>(dst + part * 32u * c.hdp);
+        for (uint32_t i = tid; i < 128u * NT; i += KvTile<NT>::TH) to[i] = reinterpret_cast<const uint4*>(img)[i];
     }
 }
 
@@ -212,8 +250,8 @@ struct Kv8AppendArgs {
 // rows into the tail. The first block's earlier rows come from the tail, which a later block of the same parity overwrites:
 // the first block's workgroup does that one too, after its own.
 template <int NT>
-__global__ void __launch_bounds__(kKvThreads) k_kv8_append(const Kv8AppendArgs A) {
-    __shared__ __align__(16) uint8_t img[1024 * NT];
+__global__ void __launch_bounds__((KvTile<NT>::TH)) k_kv8_append(const Kv8AppendArgs A) {
+    __shared__ __align__(16) uint8_t img[2048 * NT];
     __shared__ uint32_t rowmax[32];
     const Kv8Dev& c = A.c;
     const Kv8Seq& S = A.s[blockIdx.z];
@@ -228,19 +266,20 @@ __global__ void __launch_bounds__(kKvThreads) k_kv8_append(const Kv8AppendArgs A
         const uint32_t first = max(S.pos, 32u * b), last = min(end, 32u * b + 32u);   // the call's rows
         const uint64_t buf = kv_tail_buf(c, S.seq, head, b, z);
         const bool full = (b + 1u) * 32u <= end, tail = b + 1u >= bl;
+        const uint32_t from = full || last - first > kKvFew ? 32u * b : first;   // rows that matter
         KvTile<NT> T;
         const float* old = c.tail + buf * 32u * c.hdp;
 #pragma unroll
-        for (int k = 0; k < NT; ++k) {
+        for (uint32_t k = 0; k < KvTile<NT>::KU; ++k) {
             uint32_t t, d;
             kv_unit<NT>(k, t, d);
-            const uint32_t p = min(32u * b + t, last - 1u), dd = min(d, c.hd - 4u);
-            T.v[k] = *reinterpret_cast<const f4*>(p < S.pos ? old + t * c.hdp + dd : x + static_cast<uint64_t>(p - S.pos) * A.stride + dd);
+            const uint32_t p = min(max(32u * b + t, from), last - 1u), dd = min(d, c.hd - 4u);
+            T.v[k] = *reinterpret_cast<const f4*>(p < S.pos ? old + (p & 31u) * c.hdp + dd : x + static_cast<uint64_t>(p - S.pos) * A.stride + dd);
             if (d >= c.hd) T.v[k] = f4{0.0f, 0.0f, 0.0f, 0.0f};
         }
         kv_row_max<NT>(T, rowmax);   // (its barriers come after every read of the tail)
         if (full) kv_close_block<NT>(c, T, rowmax, kv_block(c, S.seq, head, b), z, img);
-        if (tail) kv_store_tail<NT>(c, T, rowmax, buf, z, first & 31u, last - 32u * b);
+        if (tail) kv_store_tail<NT>(c, T, rowmax, buf, z, first & 31u, last - 32u * b, img);
         if (b != b0 || other == b0) return;
         __syncthreads();   // the next round's row maxima and image
     }
@@ -257,7 +296,7 @@ struct Kv8ReadArgs {
 
 // One workgroup per (block, head and K or V, sequence): the block's codes in 16-byte units into LDS, rows out of it.
 template <int NT>
-__global__ void __launch_bounds__(kKvThreads) k_kv8_read(const Kv8ReadArgs A) {
+__global__ void __launch_bounds__((KvTile<NT>::TH)) k_kv8_read(const Kv8ReadArgs A) {
 #pragma clang fp contract(off)
     __shared__ __align__(16) uint8_t img[1024 * NT];
     const Kv8Dev& c = A.c;
@@ -271,12 +310,12 @@ __global__ void __launch_bounds__(kKvThreads) k_kv8_read(const Kv8ReadArgs A) {
         const uint64_t blk = kv_block(c, S.seq, head, b);
         const uint4* src = reinterpret_cast<const uint4*>(kv_codes(c, blk) + z * 32u * c.hdp);
         s = reinterpret_cast<const float*>(c.scales + blk)[z];
-        for (uint32_t i = tid; i < 64u * NT; i += kKvThreads) reinterpret_cast<uint4*>(img)[i] = src[i];
+        for (uint32_t i = tid; i < 64u * NT; i += KvTile<NT>::TH) reinterpret_cast<uint4*>(img)[i] = src[i];
         __syncthreads();
     }
     const float* old = c.tail + kv_tail_buf(c, S.seq, head, b, z) * 32u * c.hdp;
 #pragma unroll
-    for (int k = 0; k < NT; ++k) {
+    for (uint32_t k = 0; k < KvTile<NT>::KU; ++k) {
         uint32_t t, d;
         kv_unit<NT>(k, t, d);
         const uint32_t p = 32u * b + t;
@@ -1158,78 +1197,85 @@ __global__ void __launch_bounds__(kKvSelThreads) k_kv8_select(const Kv8EvictArgs
 // block, 16 bytes from its neighbours': lanes take the pieces of different tokens. A value's is a byte of every 8: lanes take
 // neighbouring dims, 16 bytes (two dims of eight tokens) a load.
 template <int NT>
-__global__ void __launch_bounds__(kKvThreads) k_kv8_gather(const Kv8EvictArgs A) {
+__global__ void __launch_bounds__((KvTile<NT>::TH)) k_kv8_gather(const Kv8EvictArgs A) {
 #pragma clang fp contract(off)
-    constexpr uint32_t kRow = 32u * NT + 8u;
-    __shared__ __align__(16) uint8_t img[1024 * NT];
+    constexpr uint32_t kRow = 32u * NT + 8u, TH = KvTile<NT>::TH;
+    __shared__ __align__(16) uint8_t img[2048 * NT];
     __shared__ __align__(16) uint8_t raw[32 * kRow];
     __shared__ uint32_t rowmax[32], s_p[32];
     __shared__ float s_s[32];
     const Kv8Dev& c = A.c;
     const vrt_kv8_move& V = A.m[blockIdx.z];
-    const uint32_t head = blockIdx.y >> 1, z = blockIdx.y & 1u, b = blockIdx.x, tid = threadIdx.x;
+    const uint32_t head = blockIdx.y >> 1, z = blockIdx.y & 1u, tid = threadIdx.x;
+    const uint32_t b = (blockIdx.x & 7u) * (gridDim.x >> 3) + (blockIdx.x >> 3);   // an XCD has neighbours, which read the same blocks
     if (32u * b >= V.keep) return;
     const uint32_t* kept = A.kept + (static_cast<uint64_t>(blockIdx.z) * c.kvh + head) * A.kept_stride;
     const uint32_t n = min(32u, V.keep - 32u * b), full = V.len >> 5;   // full blocks of the source
+    const uint64_t src0 = (static_cast<uint64_t>(V.src) * c.kvh + head) * c.nb;   // (a source is no ring)
     if (tid < 32u) {
         const uint32_t p = kept[32u * b + min(tid, n - 1u)];
         s_p[tid] = p;
-        s_s[tid] = (p >> 5) < full ? reinterpret_cast<const float*>(c.scales + kv_block(c, V.src, head, p >> 5))[z] : 0.0f;
+        s_s[tid] = reinterpret_cast<const float*>(c.scales + src0 + min(p >> 5, full ? full - 1u : 0u))[z];
     }
     __syncthreads();
+    const uint32_t top = full ? full - 1u : 0u;
     // (every load issued, at a position that is there, before the first is put down)
     if (z == 0u) {
-        constexpr uint32_t kPer = (128u * NT + kKvThreads - 1u) / kKvThreads;
+        constexpr uint32_t kPer = (128u * NT + TH - 1u) / TH;
         uint2 u[kPer];
 #pragma unroll
         for (uint32_t k = 0; k < kPer; ++k) {   // (8 dims, token)
-            const uint32_t i = min(tid + kKvThreads * k, 128u * NT - 1u), t = i & 31u, q = i >> 5, p = s_p[t];
-            const uint8_t* blk = kv_codes(c, kv_block(c, V.src, head, min(p >> 5, full - 1u)));
+            const uint32_t i = min(tid + TH * k, 128u * NT - 1u), t = i & 31u, q = i >> 5, p = s_p[t];
+            const uint8_t* blk = kv_codes(c, src0 + min(p >> 5, top));
             u[k] = *reinterpret_cast<const uint2*>(blk + kv_k_at(p & 31u, 8u * q));
         }
 #pragma unroll
         for (uint32_t k = 0; k < kPer; ++k) {
-            const uint32_t i = min(tid + kKvThreads * k, 128u * NT - 1u), t = i & 31u, q = i >> 5;
+            const uint32_t i = min(tid + TH * k, 128u * NT - 1u), t = i & 31u, q = i >> 5;
             *reinterpret_cast<uint2*>(raw + t * kRow + 8u * q) = u[k];
         }
     } else {
-        uint4 u[2 * NT];
+        constexpr uint32_t kPer = 512u * NT / TH;
+        uint4 u[kPer];
 #pragma unroll
-        for (uint32_t k = 0; k < 2u * NT; ++k) {   // (token, dims 32 jj + m and 16 on)
-            const uint32_t i = tid + kKvThreads * k, m = i & 15u, jj = (i >> 4) % NT, t = (i >> 4) / NT, p = s_p[t];
-            const uint8_t* blk = kv_codes(c, kv_block(c, V.src, head, min(p >> 5, full - 1u))) + 32u * c.hdp;
+        for (uint32_t k = 0; k < kPer; ++k) {   // (token, dims 32 jj + m and 16 on)
+            const uint32_t i = tid + TH * k, m = i & 15u, jj = (i >> 4) % NT, t = (i >> 4) / NT, p = s_p[t];
+            const uint8_t* blk = kv_codes(c, src0 + min(p >> 5, top)) + 32u * c.hdp;
             u[k] = *reinterpret_cast<const uint4*>(blk + jj * 1024u + (((p >> 2) & 3u) * 16u + m) * 16u);
         }
 #pragma unroll
-        for (uint32_t k = 0; k < 2u * NT; ++k) {
-            const uint32_t i = tid + kKvThreads * k, m = i & 15u, jj = (i >> 4) % NT, t = (i >> 4) / NT, tok = s_p[t] & 31u;
-            const bool late = tok >> 4;
-            const uint32_t sh = 8u * (tok & 3u);
-            raw[t * kRow + 32u * jj + m] = static_cast<uint8_t>((late ? u[k].y : u[k].x) >> sh);
-            raw[t * kRow + 32u * jj + 16u + m] = static_cast<uint8_t>((late ? u[k].w : u[k].z) >> sh);
+        for (uint32_t k = 0; k < kPer; ++k) {
+            const uint32_t i = tid + TH * k, m = i & 15u, jj = (i >> 4) % NT, t = (i >> 4) / NT, tok = s_p[t] & 31u;
+            const uint32_t sh = 8u * (tok & 3u) + 2u * (tok & 16u);   // its byte of the dim's eight
+            const uint64_t lo = static_cast<uint64_t>(u[k].y) << 32 | u[k].x, hi = static_cast<uint64_t>(u[k].w) << 32 | u[k].z;
+            raw[t * kRow + 32u * jj + m] = static_cast<uint8_t>(lo >> sh);
+            raw[t * kRow + 32u * jj + 16u + m] = static_cast<uint8_t>(hi >> sh);
         }
     }
     __syncthreads();
     KvTile<NT> T;
 #pragma unroll
-    for (int k = 0; k < NT; ++k) {
+    for (uint32_t k = 0; k < KvTile<NT>::KU; ++k) {
         uint32_t t, d;
         kv_unit<NT>(k, t, d);
-        T.v[k] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-        if (t >= n || d >= c.hd) continue;
-        const uint32_t p = s_p[t];
-        if ((p >> 5) < full) {
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(raw + t * kRow + d);
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(raw + t * kRow + d);
+        const float f = t < n && d < c.hd ? s_s[t] : 0.0f;
 #pragma unroll
-            for (uint32_t e = 0; e < 4u; ++e) T.v[k][e] = s_s[t] * (static_cast<float>((w >> (8u * e)) & 255u) - 128.0f);
-        } else {
-            T.v[k] = *reinterpret_cast<const f4*>(c.tail + (kv_tail_buf(c, V.src, head, p >> 5, z) * 32u + (p & 31u)) * c.hdp + d);
-        }
+        for (uint32_t e = 0; e < 4u; ++e) T.v[k][e] = f * (static_cast<float>((w >> (8u * e)) & 255u) - 128.0f);
     }
+    if (s_p[n - 1u] >> 5 >= full)   // the source's open block has some of them: the last ones
+#pragma unroll
+        for (uint32_t k = 0; k < KvTile<NT>::KU; ++k) {
+            uint32_t t, d;
+            kv_unit<NT>(k, t, d);
+            const uint32_t p = s_p[t];
+            if (t < n && d < c.hd && p >> 5 >= full)
+                T.v[k] = *reinterpret_cast<const f4*>(c.tail + (kv_tail_buf(c, V.src, head, p >> 5, z) * 32u + (p & 31u)) * c.hdp + d);
+        }
     kv_row_max<NT>(T, rowmax);
     if (n == 32u) kv_close_block<NT>(c, T, rowmax, kv_block(c, V.dst, head, b), z, img);
     if (b + 1u >= (V.keep - 1u) >> 5)   // the last block and the one before
-        kv_store_tail<NT>(c, T, rowmax, kv_tail_buf(c, V.dst, head, b, z), z, 0u, n);
+        kv_store_tail<NT>(c, T, rowmax, kv_tail_buf(c, V.dst, head, b, z), z, 0u, n, img);
 }
 
 // ---- host -----------------------------------------------------------------------------------
@@ -1345,6 +1391,8 @@ int attn_plan(const vrt_kv8_cache* c, const vrt_kv8_attn* at, const vrt_kv8_rows
 
 // Tiles of 16 rows that a prompt's wave runs together: as many as leave two waves a SIMD.
 constexpr int rows_of(int nt) { return nt <= 4 ? 4 : 2; }
+
+uint32_t tile_threads(const Kv8Dev& c) { return c.hdp >= 96u ? 512u : 256u; }   // KvTile::TH
 
 enum Kv8Kernel { kKvAppend, kKvRead, kKvToken, kKvPrompt, kKvWeights, kKvGather };
 template <int NT>
@@ -1479,7 +1527,7 @@ int kv8_append(const Kv8Dev& c, const Kv8Seq* seqs, uint32_t n, const float* k, 
         blocks = std::max(blocks, touched(seqs[i]));
     }
     if (blocks == 0u) return VRT_OK;
-    return launch(kernel_of(c, kKvAppend), dim3(blocks, 2u * c.kvh, n), kKvThreads, A, s);
+    return launch(kernel_of(c, kKvAppend), dim3(blocks, 2u * c.kvh, n), tile_threads(c), A, s);
 }
 
 int kv8_attend(Kv8AttnArgs& A, const Kv8Plan& P, void* workspace, uint32_t n, hipStream_t s) {
@@ -1517,7 +1565,7 @@ int kv8_evict(const Kv8Dev& c, const vrt_kv8_move* moves, uint32_t n, float* wei
     }
     if (keep == 0u) return VRT_OK;
     if (int rc = launch(reinterpret_cast<const void*>(&k_kv8_select), dim3(c.kvh, n), kKvSelThreads, A, s)) return rc;
-    return launch(kernel_of(c, kKvGather), dim3((keep + 31u) / 32u, 2u * c.kvh, n), kKvThreads, A, s);
+    return launch(kernel_of(c, kKvGather), dim3(((keep + 31u) / 32u + 7u) & ~7u, 2u * c.kvh, n), tile_threads(c), A, s);
 }
 
 }  // namespace vrt
@@ -1580,7 +1628,7 @@ extern "C" int vrt_kv8_read(vrt_ctx* ctx, const vrt_kv8_cache* cache, const vrt_
     if (blocks == 0u) return VRT_OK;
     OnDevice on(ctx->device);
     VRT_HIP_CHECK(on.err);
-    return launch(kernel_of(A.c, kKvRead), dim3(blocks, 2u * A.c.kvh, n_seqs), kKvThreads, A, ctx->stream);
+    return launch(kernel_of(A.c, kKvRead), dim3(blocks, 2u * A.c.kvh, n_seqs), tile_threads(A.c), A, ctx->stream);
 }
 
 extern "C" int vrt_kv8_attend_workspace(const vrt_kv8_cache* cache, const vrt_kv8_attn* attn, const vrt_kv8_rows* rows,
