@@ -37,6 +37,20 @@ __device__ __forceinline__ uint32_t kv_v_at(uint32_t t, uint32_t d) {
     return (d >> 5) * 1024u + (((t >> 2) & 3u) * 16u + (d & 15u)) * 16u + ((d >> 4) & 1u) * 8u + (t & 3u) + (t >> 4) * 4u;
 }
 
+// A launch's arguments lie in memory that nothing has cached; read where they are used, they cost a latency for every line.
+// These ask for the ones that a kernel uses all at once.
+__device__ __forceinline__ void kv_ask(const Kv8Dev& c) {
+    asm volatile("" ::"s"(c.codes), "s"(c.scales), "s"(c.tail), "s"(c.pairs), "s"(c.factor), "s"(c.nb), "s"(c.kvh), "s"(c.hd), "s"(c.hdp));
+}
+__device__ __forceinline__ void kv_ask(const Kv8Seq& s) {
+    asm volatile("" ::"s"(s.seq), "s"(s.pos), "s"(s.n), "s"(s.prefix), "s"(s.row0), "s"(s.splits), "s"(s.part0));
+}
+__device__ __forceinline__ void kv_ask(const Kv8AttnArgs& A) {
+    asm volatile("" ::"s"(A.c.codes), "s"(A.c.scales), "s"(A.c.pairs), "s"(A.c.factor), "s"(A.c.nb), "s"(A.c.kvh), "s"(A.c.hd), "s"(A.c.hdp),
+                 "s"(A.o.rows), "s"(A.o.stride), "s"(A.o.gm), "s"(A.q), "s"(A.q_stride), "s"(A.part), "s"(A.part_ml), "s"(A.heads),
+                 "s"(A.G), "s"(A.window), "s"(A.per), "s"(A.splits), "s"(A.nseq), "s"(A.scale));
+}
+
 template <int CTRL, int ROWS>
 __device__ __forceinline__ uint32_t dpp_max_u32(uint32_t v) {   // lanes outside the row mask keep their own
     return max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(static_cast<int>(v), static_cast<int>(v), CTRL, ROWS, 0xf, false)));
@@ -256,6 +270,9 @@ __global__ void __launch_bounds__((KvTile<NT>::TH)) k_kv8_append(const Kv8Append
     const Kv8Dev& c = A.c;
     const Kv8Seq& S = A.s[blockIdx.z];
     const uint32_t head = blockIdx.y >> 1, z = blockIdx.y & 1u;
+    kv_ask(c);
+    kv_ask(S);
+    asm volatile("" ::"s"(A.x[0]), "s"(A.x[1]), "s"(A.stride));
     if (S.n == 0u) return;
     const uint32_t end = S.pos + S.n, b0 = S.pos >> 5, bl = (end - 1u) >> 5;
     const float* x = A.x[z] + static_cast<uint64_t>(S.row0) * A.stride + head * c.hd;
@@ -440,13 +457,6 @@ __device__ __forceinline__ void kv_make_q(const Kv8AttnArgs& A, KvRows<NT>& X, K
             Q.q[s][1][j] = b[0], Q.q[s][1][j + 1] = b[1];
         }
 }
-template <int NT, bool CAP>
-__device__ __forceinline__ void kv_load_q(const Kv8AttnArgs& A, const Kv8Seq& S, uint32_t kvh, uint32_t r0, KvQuery<NT>& Q, float& f) {
-    KvRows<NT> X;
-    kv_load_rows<NT>(A, S, kvh, r0, X);
-    kv_make_q<NT, CAP>(A, X, Q, f);
-}
-
 // What a wave holds of RT tiles of 16 rows (lane l: row l % 16 of each). The outputs are transposed too (dims 16 t + 4 (l / 16) + e), in
 // units of 2^(eR - 9).
 constexpr float kKvGrow = 6.0f;   // weights may pass 1 by 2^6 before the reference maximum follows
@@ -689,8 +699,10 @@ __device__ __forceinline__ void kv_open(const Kv8AttnArgs& A, const Kv8Seq& S, u
 #pragma unroll
     for (uint32_t e = 0; e < 8u; ++e) {
         const bool y = kv_token(e) < live;
-        ks[e] = y ? c.factor[kb * 32u + kv_token(e)] : 0.0f;
-        vs[e] = y ? c.factor[vb * 32u + kv_token(e)] : 0.0f;
+        ks[e] = c.factor[kb * 32u + kv_token(e)];
+        vs[e] = c.factor[vb * 32u + kv_token(e)];
+        ks[e] = y ? ks[e] : 0.0f;
+        vs[e] = y ? vs[e] : 0.0f;
         keep[e >> 1] = (e & 1u ? keep[e >> 1] : 0u) | (y ? 0xffffu << (16u * (e & 1u)) : 0u);
     }
     f4 s[RT][2];
@@ -712,6 +724,78 @@ __device__ __forceinline__ void kv_open(const Kv8AttnArgs& A, const Kv8Seq& S, u
             W.acc[k][t] = KV_MFMA(d, ph[k], W.acc[k][t]);
         }
     }
+}
+
+// The same by a workgroup's four waves together (one tile of rows): a wave's quarter of the dims goes into its part of the
+// scores, which meet in LDS (xch: [4][2][64] f4), and out of its quarter of the values, into its own sums; `owner` counts the weights.
+// By one wave alone, with 64 KB to read, it was half of a step's time at short histories.
+template <int NT, bool CAP>
+__device__ __forceinline__ void kv_open_all(const Kv8AttnArgs& A, const Kv8Seq& S, uint32_t kvh, uint32_t b, KvWave<NT, 1>& W, bool owner,
+                                            f4* xch, float* dump) {
+    constexpr int NK = (NT + 3) / 4, NV = (2 * NT + 3) / 4;
+    const Kv8Dev& c = A.c;
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), live = S.pos + S.n - 32u * b;
+    const uint64_t kb = kv_tail_buf(c, S.seq, kvh, b, 0u), vb = kb + 1u;
+    const h8* kp = reinterpret_cast<const h8*>(c.pairs + kb * 64u * c.hdp) + lane;
+    const uint4* vp = reinterpret_cast<const uint4*>(c.pairs + vb * 64u * c.hdp) + lane;
+    h8 k[NK][2][2];
+    uint4 v[NV][2];
+#pragma unroll
+    for (int i = 0; i < NK; ++i)
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (uint32_t part = 0; part < 2u; ++part)
+                k[i][half][part] = kp[64u * (2u * min(wave + 4u * i, NT - 1u) + half) + part * 4u * c.hdp];
+    float ks[8], vs[8];
+    uint32_t keep[4];   // of the values' operand: halves 2 i and 2 i + 1
+#pragma unroll
+    for (uint32_t e = 0; e < 8u; ++e) {
+        const bool y = kv_token(e) < live;
+        ks[e] = c.factor[kb * 32u + kv_token(e)];
+        vs[e] = c.factor[vb * 32u + kv_token(e)];
+        ks[e] = y ? ks[e] : 0.0f;
+        vs[e] = y ? vs[e] : 0.0f;
+        keep[e >> 1] = (e & 1u ? keep[e >> 1] : 0u) | (y ? 0xffffu << (16u * (e & 1u)) : 0u);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (uint32_t part = 0; part < 2u; ++part) v[i][part] = vp[64u * min(wave + 4u * i, 2u * NT - 1u) + part * 4u * c.hdp];
+    __builtin_amdgcn_sched_barrier(0);
+    f4 s[1][2] = {{{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}}};
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+        if (static_cast<uint32_t>(t & 3) == wave)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                s[0][half] = KV_MFMA(k[t >> 2][half][0], W.query(0, t, 0), s[0][half]);
+                s[0][half] = KV_MFMA(k[t >> 2][half][1], W.query(0, t, 0), s[0][half]);
+                s[0][half] = KV_MFMA(k[t >> 2][half][0], W.query(0, t, 1), s[0][half]);
+            }
+#pragma unroll
+    for (int half = 0; half < 2; ++half) xch[(wave * 2u + half) * 64u + lane] = s[0][half];
+    __syncthreads();
+#pragma unroll
+    for (uint32_t half = 0; half < 2u; ++half)
+        s[0][half] = (xch[half * 64u + lane] + xch[(2u + half) * 64u + lane]) + (xch[(4u + half) * 64u + lane] + xch[(6u + half) * 64u + lane]);
+    h8 ph[1], pl[1];
+    const float before = W.l[0];
+    const float m0 = W.m[0];
+    kv_soft<NT, 1, CAP, true>(A, S, b, true, s, ks, vs, W, ph, pl, owner ? dump : nullptr);
+    if (!owner) W.l[0] = before * (W.m[0] == m0 ? 1.0f : __builtin_amdgcn_exp2f(m0 - W.m[0]));
+#pragma unroll
+    for (int t = 0; t < 2 * NT; ++t)
+        if (static_cast<uint32_t>(t & 3) == wave) {
+            uint4 x = v[t >> 2][0], y = v[t >> 2][1];
+            x.x &= keep[0], x.y &= keep[1], x.z &= keep[2], x.w &= keep[3];
+            y.x &= keep[0], y.y &= keep[1], y.z &= keep[2], y.w &= keep[3];
+            const h8 a = __builtin_bit_cast(h8, x), d = __builtin_bit_cast(h8, y);
+            W.acc[0][t] = KV_MFMA(a, ph[0], W.acc[0][t]);
+            W.acc[0][t] = KV_MFMA(a, pl[0], W.acc[0][t]);
+            W.acc[0][t] = KV_MFMA(d, ph[0], W.acc[0][t]);
+        }
+    __syncthreads();   // xch is the waves' meeting place too
 }
 
 // Whether some row at positions pmin .. pmax does not see all of the full block b.
@@ -750,7 +834,7 @@ __device__ __forceinline__ void kv_row_done(const Kv8AttnArgs& A, uint32_t row, 
 // scores, which leaves those registers to the queries); the first block's before start() makes the queries.
 template <int NT, int RT, bool CAP, class Start>
 __device__ __forceinline__ void kv_run(const Kv8AttnArgs& A, const Kv8Seq& S, uint32_t kvh, const KvSpan& sp, uint32_t pmin, uint32_t pmax,
-                                       uint32_t i0, uint32_t i1, KvWave<NT, RT>& W, float* dump, Start start) {
+                                       uint32_t i0, uint32_t i1, KvWave<NT, RT>& W, f4* xch, float* dump, Start start) {
     const Kv8Dev& c = A.c;
     auto block = [&](uint32_t i) { return i < sp.n_pre ? i : sp.lo + (i - sp.n_pre); };
     const uint32_t last = block(sp.n - 1u);
@@ -785,7 +869,13 @@ __device__ __forceinline__ void kv_run(const Kv8AttnArgs& A, const Kv8Seq& S, ui
         if (RT == 1) kv_load<NT>(c, blk, 1u, V);
         __builtin_amdgcn_sched_barrier(0);
     }
-    if (open && i == sp.n - 1u && i < i1) kv_open<NT, RT, CAP>(A, S, kvh, last, W, dump ? dump + 32u * (i - i0) : nullptr);
+    const bool mine = open && i == sp.n - 1u && i < i1;
+    float* const to = dump ? dump + 32u * (i - i0) : nullptr;
+    if constexpr (RT == 1) {
+        if (open && i1 == sp.n) kv_open_all<NT, CAP>(A, S, kvh, last, W, mine, xch, to);   // all waves of the workgroup
+    } else if (mine) {
+        kv_open<NT, RT, CAP>(A, S, kvh, last, W, to);
+    }
 }
 
 // One workgroup per (split of a unit's blocks, head, sequence), its waves taking every fourth block and meeting in LDS, eight rows
@@ -796,13 +886,16 @@ __device__ __forceinline__ void kv_run(const Kv8AttnArgs& A, const Kv8Seq& S, ui
 template <int NT, int RT, bool CAP>
 __global__ void __launch_bounds__(kKvThreads, 2) k_kv8_attn(const Kv8AttnArgs A) {
     constexpr uint32_t HDP = 32u * NT, C4 = HDP / 4u;
-    constexpr uint32_t kMeet = 4u * 8u * C4, kQ = RT > 1 ? RT * NT * 128u : 0u;   // units of 16 bytes: the waves' outputs; queries
-    __shared__ __align__(16) f4 s_buf[kMeet > kQ ? kMeet : kQ];
+    // units of 16 bytes: the waves' outputs; the prompts' queries, or the waves' shares of the open block's scores
+    constexpr uint32_t kMeet = 4u * 8u * C4, kOther = RT > 1 ? RT * NT * 128u : 4u * 2u * 64u;
+    __shared__ __align__(16) f4 s_buf[kMeet > kOther ? kMeet : kOther];
     __shared__ float s_m[4][16 * RT], s_l[4][16 * RT], s_f[16 * RT];
     f4* const s_acc = s_buf;   // [4][8 C4], after the queries' last use
+    kv_ask(A);
     const uint32_t pairs = A.nseq * A.c.kvh, pair = blockIdx.x % pairs, rest = blockIdx.x / pairs;
     const uint32_t kvh = pair % A.c.kvh, split = rest % A.splits;
     const Kv8Seq& S = A.s[pair / A.c.kvh];
+    kv_ask(S);
     const uint32_t R = S.n * A.G, units = (R + 16u * RT - 1u) / (16u * RT), at = rest / A.splits;
     if (at >= units || split >= S.splits) return;
     const uint32_t unit = A.fold && at >= units / 2u ? at - units / 2u : units - 1u - at;
@@ -816,15 +909,18 @@ __global__ void __launch_bounds__(kKvThreads, 2) k_kv8_attn(const Kv8AttnArgs A)
     float* dump = nullptr;   // this lane's row of the unit's scores
     if (RT == 1 && A.scores && m16 < rows) dump = A.scores + (place * A.lines + m16) * 32u * A.per + 32u * wave + 4u * g;
     KvWave<NT, RT> W;
-    kv_run<NT, RT, CAP>(A, S, kvh, sp, pmin, pmax, i0 + wave, i1, W, dump, [&]() {
+    KvRows<NT> X;
+    if (RT == 1 || wave < RT) kv_load_rows<NT>(A, S, kvh, r0 + (RT == 1 ? 0u : 16u * wave), X);   // (several tiles: one a wave)
+    __builtin_amdgcn_sched_barrier(0);
+    kv_run<NT, RT, CAP>(A, S, kvh, sp, pmin, pmax, i0 + wave, i1, W, s_buf, dump, [&]() {
         if constexpr (RT == 1) {
-            kv_load_q<NT, CAP>(A, S, kvh, r0, W.q, W.f[0]);
+            kv_make_q<NT, CAP>(A, X, W.q, W.f[0]);
         } else {
             h8* sq = reinterpret_cast<h8*>(s_buf) + lane;
-            if (wave < RT) {   // a tile each
+            if (wave < RT) {
                 KvQuery<NT> Q;
                 float f;
-                kv_load_q<NT, CAP>(A, S, kvh, r0 + 16u * wave, Q, f);
+                kv_make_q<NT, CAP>(A, X, Q, f);
 #pragma unroll
                 for (int s = 0; s < NT; ++s)
 #pragma unroll
@@ -894,6 +990,8 @@ __global__ void __launch_bounds__(kKvThreads) k_kv8_join(const Kv8AttnArgs A) {
     const Kv8Seq& S = A.s[blockIdx.z];
     const Kv8Dev& c = A.c;
     const uint32_t kvh = blockIdx.y, R = S.n * A.G, U = A.unit, tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
+    kv_ask(A);
+    kv_ask(S);
     const uint32_t join_rows = A.splits > 1u ? A.rows_most : 0u;
     if (blockIdx.x < join_rows) {
         const uint32_t r = blockIdx.x, unit = r / U, rr = r - unit * U;
@@ -968,16 +1066,21 @@ __global__ void __launch_bounds__(kKvThreads) k_kv8_join(const Kv8AttnArgs A) {
 
 // Prompts' accumulated weights: one workgroup per (block of positions, head, sequence), its waves taking every eighth of the 16-row
 // tiles that see the block; the scores once more, against the rows' final maxima and sums. A tile's rows are loaded while the
-// one before is worked on.
-constexpr uint32_t kKvWeightWaves = 8;
+// one before is worked on. The blocks that the most rows see come first, and every other 256 of the workgroups the other way
+// round, so that the longest meets the shortest on its CU: 3 prompts of 2048 positions, 8 heads of 64, take 72 us, in the grid's
+// own order 129 us. What remains is the vector unit's (a row's halves are made once for every block), not memory's.
+constexpr uint32_t kKvWeightWaves = 8, kKvCus = 256;
 template <int NT, bool CAP>
 __global__ void __launch_bounds__(64 * kKvWeightWaves, 2) k_kv8_weights(const Kv8AttnArgs A) {
     __shared__ float s_w[kKvWeightWaves][32];
-    const Kv8Seq& S = A.s[blockIdx.z];
+    const uint32_t pairs = gridDim.y * gridDim.z, id = (blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
+    const uint32_t in = id % kKvCus, first = id - in, left = min(pairs * gridDim.x - first, kKvCus);
+    const uint32_t nth = first + (first & kKvCus ? left - 1u - in : in), pair = nth % pairs;
+    const Kv8Seq& S = A.s[pair / A.c.kvh];
     const Kv8Dev& c = A.c;
-    const uint32_t kvh = blockIdx.y, m16 = threadIdx.x & 15u;
+    const uint32_t kvh = pair % A.c.kvh, m16 = threadIdx.x & 15u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t len = S.pos + S.n, R = S.n * A.G, b = blockIdx.x, p0 = 32u * b, p1 = p0 + 31u;
+    const uint32_t len = S.pos + S.n, R = S.n * A.G, b = nth / pairs, p0 = 32u * b, p1 = p0 + 31u;
     if (S.n == 0u || p0 >= len) return;
     const bool open = p1 >= len;
     float w[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
@@ -986,7 +1089,9 @@ __global__ void __launch_bounds__(64 * kKvWeightWaves, 2) k_kv8_weights(const Kv
     const uint64_t kb = kv_tail_buf(c, S.seq, kvh, b, 0u);
     if (open) {
 #pragma unroll
-        for (uint32_t e = 0; e < 8u; ++e) ks[e] = p0 + kv_token(e) < len ? c.factor[kb * 32u + kv_token(e)] : 0.0f;
+        for (uint32_t e = 0; e < 8u; ++e) ks[e] = c.factor[kb * 32u + kv_token(e)];
+#pragma unroll
+        for (uint32_t e = 0; e < 8u; ++e) ks[e] = p0 + kv_token(e) < len ? ks[e] : 0.0f;
     } else {
         const uint64_t blk = kv_block(c, S.seq, kvh, b);
         kv_load<NT>(c, blk, 0u, K);
@@ -1462,6 +1567,7 @@ Kv8Dev kv8_view(const Kv8Sizes& z, void* data, uint32_t kv_heads, uint32_t head_
 // A unit's blocks are split where there are too few units: into about 512 workgroups (two a CU), of four blocks (one a wave) at
 // least. Prompts with as many units as that are not split: their outputs would be written and read once more.
 constexpr uint64_t kKvSplits = 512;
+constexpr uint32_t kKvWhole = 24;
 
 Kv8Plan kv8_plan(Kv8AttnArgs& A, uint32_t kvh, uint32_t hdp, uint32_t n, uint64_t rows, bool scored) {
     Kv8Plan P{};
@@ -1476,15 +1582,18 @@ Kv8Plan kv8_plan(Kv8AttnArgs& A, uint32_t kvh, uint32_t hdp, uint32_t n, uint64_
     A.unit = A.prompt ? 16u * rows_of(static_cast<int>(hdp / 32u)) : 16u;
     A.lines = std::min(A.unit, std::max(1u, A.rows_most));
     uint64_t units_all = 0, blocks = 0;   // of all units and heads; a prompt's queries see half of its own on average
+    uint32_t most = 1;                    // blocks of a unit
     for (uint32_t i = 0; i < n; ++i) {
         const Kv8Seq& s = A.s[i];
-        const uint32_t most = most_blocks(s, A.window, A.unit);
+        const uint32_t nb = most_blocks(s, A.window, A.unit);
+        most = std::max(most, nb);
         const uint64_t units = static_cast<uint64_t>((s.n * A.G + A.unit - 1u) / A.unit) * kvh;
         units_all += units;
-        blocks += units * (s.prefix ? most : std::min(most, (s.pos + (s.n + 1u) / 2u + 31u) / 32u));
+        blocks += units * (s.prefix ? nb : std::min(nb, (s.pos + (s.n + 1u) / 2u + 31u) / 32u));
     }
     uint64_t per = std::max<uint64_t>(4u, (blocks + kKvSplits - 1u) / kKvSplits);
     if (A.prompt && units_all >= kKvSplits / 2u) per = VRT_KV8_MAX_CTX / 32u + 4u;
+    else if (most <= kKvWhole) per = most;
     A.fold = A.prompt && units_all <= kKvSplits;
     A.per = static_cast<uint32_t>((per + 3u) & ~3ull);
     A.splits = 1u;
