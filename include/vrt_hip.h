@@ -195,11 +195,11 @@ typedef struct vrt_kv8_attn {
     uint32_t heads;        /* query heads, a multiple of kv_heads: head h reads kv head h / (heads / kv_heads) */
     uint32_t window;       /* positions a query sees back, its own included (0: all) */
     float scale;           /* of the scores q . k */
-    float softcap;         /* > 0: scores become softcap tanh(score / softcap); 0: off */
+    float softcap;         /* at least 1e-6: scores become softcap tanh(score / softcap); 0: off */
 } vrt_kv8_attn;
 
 /* Attention of the last n positions of each sequence over its cache (which holds all pos + n of
- * them: append first): q and out are rows of [heads][head_dim]. The query at position i sees position j
+ * them: append first): q and out are rows of [heads][head_dim] that do not overlap. The query at position i sees position j
  * if j < prefix, or if j <= i and i - j < window (a prefix is seen by every query: the bidirectional part of a
  * prompt, or positions that stay in sight past a window). The softmax runs in fp32.
  * A key or value that is not finite (in a full block: any of the block) makes the outputs of the queries that see it NaN.

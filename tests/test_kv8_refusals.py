@@ -123,6 +123,24 @@ def test_attend_arguments():
     _refused(_attend(rows=r, wout=A, ws=A + 64), "workspace")
 
 
+def test_attend_softcap_has_a_reciprocal():
+    _refused(_attend(cap=1e-40), "softcap")
+    _refused(_attend(cap=9e-7), "softcap")
+
+
+def test_attend_grid():
+    """Every sequence of a call has as many workgroups as its longest: 64 rows of a head each, fewer than 2^24 in all."""
+    big, n = _cache(max_seqs=64, max_ctx=1 << 26), C.c_uint64()
+    at = vrt.Kv8Attn(4, 0, 1.0, 0.0)
+    rows = lambda m: _rows([(i, 0, m if i == 0 else 0, 0) for i in range(64)])  # noqa: E731
+    r = rows(1 << 22)    # 2 heads of 2^17 units, 64 times
+    _refused(vrt.lib().vrt_kv8_attend_workspace(C.byref(big), C.byref(at), vrt.ptr(r), 64, 0, C.byref(n)), "too many rows")
+    r = rows((1 << 22) - 64)
+    vrt.check(vrt.lib().vrt_kv8_attend_workspace(C.byref(big), C.byref(at), vrt.ptr(r), 64, 0, C.byref(n)))
+    r = rows(1 << 22)
+    vrt.check(vrt.lib().vrt_kv8_attend_workspace(C.byref(big), C.byref(at), vrt.ptr(r), 1, 0, C.byref(n)))
+
+
 def test_read_arguments():
     def read(rows, lens=None, cache=None, k=A):
         r = _rows(rows)

@@ -1470,7 +1470,9 @@ int attn_plan(const vrt_kv8_cache* c, const vrt_kv8_attn* at, const vrt_kv8_rows
     VRT_REQUIRE(at->heads >= 1u && at->heads <= 65535u && at->heads % c->kv_heads == 0u,
                 "%s: heads must be a multiple of kv_heads, at most 65535", who);
     VRT_REQUIRE(std::isfinite(at->scale), "%s: scale is not finite", who);
-    VRT_REQUIRE(std::isfinite(at->softcap) && at->softcap >= 0.0f, "%s: softcap must be finite, not negative", who);
+    // (its reciprocal times a score's factor is to stay a number)
+    VRT_REQUIRE(std::isfinite(at->softcap) && (at->softcap == 0.0f || at->softcap >= 1e-6f),
+                "%s: softcap must be finite, 0 or at least 1e-6", who);
     if (int rc = check_rows(c, rows, n, who, A.s, total)) return rc;
     A.heads = at->heads;
     A.G = at->heads / c->kv_heads;
@@ -1489,8 +1491,10 @@ int attn_plan(const vrt_kv8_cache* c, const vrt_kv8_attn* at, const vrt_kv8_rows
         VRT_REQUIRE(!scored || len <= c->max_ctx, "%s: weights need pos + n <= max_ctx", who);
         items += (static_cast<uint64_t>(s.n) * A.G + 15u) / 16u * c->kv_heads;
     }
-    VRT_REQUIRE(*total * A.G <= 0x3fffffffu && items <= 0x3fffffu, "%s: too many rows", who);   // grids of 2^31 workgroups
+    VRT_REQUIRE(*total * A.G <= 0x3fffffffu && items <= 0x3fffffu, "%s: too many rows", who);
     *P = kv8_plan(A, c->kv_heads, z.hdp, n, *total, scored);
+    // a grid has fewer than 2^32 threads, and as many workgroups for every sequence as for the longest
+    VRT_REQUIRE(static_cast<uint64_t>(P->units) * A.splits * c->kv_heads * n < (1ull << 32) / kKvThreads, "%s: too many rows", who);
     return VRT_OK;
 }
 
@@ -1615,7 +1619,8 @@ Kv8Plan kv8_plan(Kv8AttnArgs& A, uint32_t kvh, uint32_t hdp, uint32_t n, uint64_
     return P;
 }
 
-// Blocks a sequence's unit and head: at most ceil(max_ctx / 32); splits: at most blocks / per + 1, all blocks / per at most kKvSplits.
+// Of calls with one row a sequence and at most 32 query heads a kv head. Blocks of a sequence's unit and head: at most
+// ceil(max_ctx / 32); splits: at most blocks / per + 1, all blocks / per at most kKvSplits.
 uint64_t kv8_workspace_most(uint32_t seqs, uint32_t max_ctx, uint32_t heads, uint32_t kvh, uint32_t hdp, bool scored) {
     const uint64_t items = static_cast<uint64_t>(seqs) * kvh * ((heads / kvh + 15u) / 16u), blocks = items * ((max_ctx + 31u) / 32u);
     const uint64_t per = (std::max<uint64_t>(4u, (blocks + kKvSplits - 1u) / kKvSplits) + 3u) & ~3ull;
