@@ -163,6 +163,7 @@ CASES = [
     (2, 1, 192, [(97, 60)], 0, 0.0, 1000),                      # all see all
     (5, 5, 224, [(130, 40)], 100, 0.0, 3),
     (16, 2, 64, [(1200, 515)], 0, 30.0, 0),
+    (8, 4, 32, [(1050, 40), (600, 600), (33, 33), (1056, 70), (900, 20)], 0, 0.0, 0),   # 660 blocks' weights
 ]
 
 

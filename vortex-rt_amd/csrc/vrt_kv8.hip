@@ -94,7 +94,8 @@ __device__ __forceinline__ float kv_round(float x, float s, float inv) {
 
 // A workgroup's 32 rows of one head and block: KU float4 a thread (unit tid + TH k: token unit / (8 NT), dims 4 (unit % (8 NT)) ..;
 // zeros past hd; the last unit again past the end), their largest magnitude, scale, codes, in operand order through an LDS
-// image. Of 96 dims and more, 512 threads: with 256 a thread's share of 256 dims takes 217 registers, or spills.
+// image. Of 96 dims and more, 512 threads: with 256 a thread's share of 256 dims takes 217 registers, or spills; with 1024
+// from 160 dims on an eviction's tiles take 137 us for 125 and a read's 65 for 52 (64 sequences, 2048 positions of 256 dims).
 template <int NT>
 struct KvTile {
     static constexpr uint32_t TH = NT >= 3 ? 512u : 256u, KU = (256u * NT + TH - 1u) / TH;
@@ -174,7 +175,8 @@ __device__ __forceinline__ void kv_close_block(const Kv8Dev& c, const KvTile<NT>
     if (tid == 0u) reinterpret_cast<float*>(c.scales + block)[z] = s;
 }
 
-constexpr uint32_t kKvFew = 2;   // rows whose pairs are scattered
+// Rows whose pairs are scattered: a step's one, as a buffer of 64 KB would be written for it; more go through LDS.
+constexpr uint32_t kKvFew = 2;
 
 // Halves of a row's pair in operand order: K by four dims, V by one.
 __device__ __forceinline__ uint32_t kv_k_half(uint32_t t, uint32_t d) {
@@ -882,7 +884,10 @@ __device__ __forceinline__ void kv_run(const Kv8AttnArgs& A, const Kv8Seq& S, ui
 // at a time. A unit is 16 RT rows: 16 for single tokens (memory's time: two workgroups a CU hold 16 KB a wave in
 // flight); more for prompts, where a block's codes become halves once for all of a wave's rows. A sequence's units come the
 // longest first, so that what is left at the end is short (or, where all run at once, so that a CU's two are as long
-// together as any other's); the (head, sequence)s side by side: eight of them or a multiple have an XCD's L2 each.
+// together as any other's: a prompt of 4096 rows 95 us, in descending order 101, interleaved 113); the (head, sequence)s side by
+// side: eight of them or a multiple have an XCD's L2 each.
+// Measured: 64 sequences of up to 8 K, one head of 256: 39 us, 3.5 TB/s of codes; 2 of 128 K, 8 heads of 128: 105 us, 4.4 TB/s;
+// a prompt of 4096 rows, 4 heads of 256: 95 us. Prompts are the vector unit's (exponentials, maxima, halves of the weights), tokens memory's.
 template <int NT, int RT, bool CAP>
 __global__ void __launch_bounds__(kKvThreads, 2) k_kv8_attn(const Kv8AttnArgs A) {
     constexpr uint32_t HDP = 32u * NT, C4 = HDP / 4u;
@@ -1569,8 +1574,11 @@ Kv8Dev kv8_view(const Kv8Sizes& z, void* data, uint32_t kv_heads, uint32_t head_
 }
 
 // A unit's blocks are split where there are too few units: into about 512 workgroups (two a CU), of four blocks (one a wave) at
-// least. Prompts with as many units as that are not split: their outputs would be written and read once more.
+// least. Into 512, 1024 and 2048: 64 sequences of 8 K, one head of 256, 43, 48 and 52 us; 2 of 128 K, 8 heads of 128, 109, 101 and 94
+// but 5, 7 and 10 in the join. Prompts with a unit for every CU are not split: their outputs would be written and read once more.
 constexpr uint64_t kKvSplits = 512;
+// Units of this many blocks or fewer, six a wave, stay whole: 64 sequences in a window of 512 (17 blocks) take 15 to 18 us whole,
+// and split by five 15 and 4 in the join.
 constexpr uint32_t kKvWhole = 24;
 
 Kv8Plan kv8_plan(Kv8AttnArgs& A, uint32_t kvh, uint32_t hdp, uint32_t n, uint64_t rows, bool scored) {
@@ -1582,7 +1590,7 @@ Kv8Plan kv8_plan(Kv8AttnArgs& A, uint32_t kvh, uint32_t hdp, uint32_t n, uint64_
         A.rows_most = std::max(A.rows_most, A.s[i].n * A.G);
     }
     A.nseq = n;
-    A.prompt = rows * A.G > 32ull * active;
+    A.prompt = rows * A.G > 32ull * active;   // from three of a token's tiles on; below, most of a prompt's tiles would be empty
     A.unit = A.prompt ? 16u * rows_of(static_cast<int>(hdp / 32u)) : 16u;
     A.lines = std::min(A.unit, std::max(1u, A.rows_most));
     uint64_t units_all = 0, blocks = 0;   // of all units and heads; a prompt's queries see half of its own on average
