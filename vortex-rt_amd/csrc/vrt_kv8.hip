@@ -127,8 +127,22 @@ __device__ __forceinline__ void kv_row_max(const KvTile<NT>& x, uint32_t* rowmax
     __syncthreads();
 }
 
+// Places (bytes) of operand-order images in LDS. A row's neighbouring values are 16 bytes apart, or 256: in order, all 64 lanes
+// of a row meet in 4 or 8 of the 64 banks. Mixed, units of 16 bytes change places among the 16 of their 256 bytes, by the bits
+// that tell a row's units apart; reads of units in order still have all banks. An eviction's gather, with an image more, takes
+// 100 us for 125 (64 sequences, 2048 positions of 256 dims). Append, which waits for memory and needs the registers, leaves them in
+// order: 4 fills of 8192 positions, 2 heads of 256, take 44 us, with mixed tails 62.
+template <bool MIX>
+__device__ __forceinline__ uint32_t kv_img(uint32_t z, uint32_t at) {
+    return !MIX ? at : z ? at ^ (at >> 6 & 0x30u) : at ^ (at >> 4 & 0xf0u);
+}
+template <bool MIX>
+__device__ __forceinline__ uint32_t kv_img_pairs(uint32_t z, uint32_t at) {   // of halves
+    return !MIX ? at : z ? at ^ (at >> 6 & 0x30u) : at ^ (at >> 4 & 0x30u) ^ (at >> 5 & 0xc0u);
+}
+
 // A full block's codes and scale.
-template <int NT>
+template <int NT, bool MIX>
 __device__ __forceinline__ void kv_close_block(const Kv8Dev& c, const KvTile<NT>& x, const uint32_t* rowmax, uint64_t block, uint32_t z,
                                                uint8_t* img) {
     const uint32_t tid = threadIdx.x, m = wave_max_u32(rowmax[tid & 31u]);
@@ -163,15 +177,15 @@ __device__ __forceinline__ void kv_close_block(const Kv8Dev& c, const KvTile<NT>
         uint32_t t, d;
         kv_unit<NT>(k, t, d);
         if (z == 0u) {
-            *reinterpret_cast<uint32_t*>(img + kv_k_at(t, d)) = w[k];
+            *reinterpret_cast<uint32_t*>(img + kv_img<MIX>(0u, kv_k_at(t, d))) = w[k];
         } else {
 #pragma unroll
-            for (uint32_t e = 0; e < 4u; ++e) img[kv_v_at(t, d + e)] = static_cast<uint8_t>(w[k] >> (8u * e));
+            for (uint32_t e = 0; e < 4u; ++e) img[kv_img<MIX>(1u, kv_v_at(t, d + e))] = static_cast<uint8_t>(w[k] >> (8u * e));
         }
     }
     __syncthreads();
     uint4* dst = reinterpret_cast<uint4*>(kv_codes(c, block) + z * 32u * c.hdp);
-    for (uint32_t i = tid; i < 64u * NT; i += KvTile<NT>::TH) dst[i] = reinterpret_cast<const uint4*>(img)[i];
+    for (uint32_t i = tid; i < 64u * NT; i += KvTile<NT>::TH) dst[i] = *reinterpret_cast<const uint4*>(img + kv_img<MIX>(z, 16u * i));
     if (tid == 0u) reinterpret_cast<float*>(c.scales + block)[z] = s;
 }
 
@@ -190,7 +204,7 @@ __device__ __forceinline__ uint32_t kv_v_half(uint32_t t, uint32_t d) {
 // The halves of a row with a value that is not finite are zeros, so that what is masked adds nothing; its factor says so.
 // A few rows' pairs are scattered (a value's halves are 2-byte stores, 16 bytes apart); of more, the whole buffer's go
 // through LDS: scattered, 32 rows of 256 took a workgroup 7 us. img: 2048 NT bytes.
-template <int NT>
+template <int NT, bool MIX>
 __device__ __forceinline__ void kv_store_tail(const Kv8Dev& c, const KvTile<NT>& x, const uint32_t* rowmax, uint64_t buf, uint32_t z,
                                               uint32_t r0, uint32_t r1, uint8_t* img) {
     typedef _Float16 h4 __attribute__((ext_vector_type(4)));
@@ -232,7 +246,6 @@ __device__ __forceinline__ void kv_store_tail(const Kv8Dev& c, const KvTile<NT>&
         }
         return;
     }
-    _Float16* const im = reinterpret_cast<_Float16*>(img);
 #pragma unroll 1
     for (uint32_t part = 0; part < 2u; ++part) {
         __syncthreads();
@@ -244,14 +257,14 @@ __device__ __forceinline__ void kv_store_tail(const Kv8Dev& c, const KvTile<NT>&
             h4 pair[2];
             row(k, t, pair);
             const h4 v = part ? pair[1] : pair[0];
-            if (z == 0u) *reinterpret_cast<h4*>(im + kv_k_half(t, d)) = v;
+            if (z == 0u) *reinterpret_cast<h4*>(img + kv_img_pairs<MIX>(0u, 2u * kv_k_half(t, d))) = v;
             else
 #pragma unroll
-                for (uint32_t e = 0; e < 4u; ++e) im[kv_v_half(t, d + e)] = v[e];
+                for (uint32_t e = 0; e < 4u; ++e) *reinterpret_cast<_Float16*>(img + kv_img_pairs<MIX>(1u, 2u * kv_v_half(t, d + e))) = v[e];
         }
         __syncthreads();
         uint4* const to = reinterpret_cast<uint4*>(dst + part * 32u * c.hdp);
-        for (uint32_t i = tid; i < 128u * NT; i += KvTile<NT>::TH) to[i] = reinterpret_cast<const uint4*>(img)[i];
+        for (uint32_t i = tid; i < 128u * NT; i += KvTile<NT>::TH) to[i] = *reinterpret_cast<const uint4*>(img + kv_img_pairs<MIX>(z, 16u * i));
     }
 }
 
@@ -297,8 +310,8 @@ __global__ void __launch_bounds__((KvTile<NT>::TH)) k_kv8_append(const Kv8Append
             if (d >= c.hd) T.v[k] = f4{0.0f, 0.0f, 0.0f, 0.0f};
         }
         kv_row_max<NT>(T, rowmax);   // (its barriers come after every read of the tail)
-        if (full) kv_close_block<NT>(c, T, rowmax, kv_block(c, S.seq, head, b), z, img);
-        if (tail) kv_store_tail<NT>(c, T, rowmax, buf, z, first & 31u, last - 32u * b, img);
+        if (full) kv_close_block<NT, false>(c, T, rowmax, kv_block(c, S.seq, head, b), z, img);
+        if (tail) kv_store_tail<NT, false>(c, T, rowmax, buf, z, first & 31u, last - 32u * b, img);
         if (b != b0 || other == b0) return;
         __syncthreads();   // the next round's row maxima and image
     }
@@ -1383,9 +1396,9 @@ __global__ void __launch_bounds__((KvTile<NT>::TH)) k_kv8_gather(const Kv8EvictA
                 T.v[k] = *reinterpret_cast<const f4*>(c.tail + (kv_tail_buf(c, V.src, head, p >> 5, z) * 32u + (p & 31u)) * c.hdp + d);
         }
     kv_row_max<NT>(T, rowmax);
-    if (n == 32u) kv_close_block<NT>(c, T, rowmax, kv_block(c, V.dst, head, b), z, img);
+    if (n == 32u) kv_close_block<NT, true>(c, T, rowmax, kv_block(c, V.dst, head, b), z, img);
     if (b + 1u >= (V.keep - 1u) >> 5)   // the last block and the one before
-        kv_store_tail<NT>(c, T, rowmax, kv_tail_buf(c, V.dst, head, b, z), z, 0u, n, img);
+        kv_store_tail<NT, true>(c, T, rowmax, kv_tail_buf(c, V.dst, head, b, z), z, 0u, n, img);
 }
 
 // ---- host -----------------------------------------------------------------------------------
